@@ -1,0 +1,40 @@
+// 8-bit activation blocks (esr_act8.hip, esr_gn.hip, esr_wgrad8.hip; layout in include/esr_amd.h).
+//
+// A block is 32 consecutive channels of one pixel (the last block of a pixel may be shorter).  Its values share one
+// power-of-two step 2^(e - 132), e in [0, 254], the smallest with 127·step >= max|x|; a value is code·step, code in
+// [-127, 127].  A power of two because code·step is then exact in fp32 (and, with 7 significant bits, in f16 / bf16,
+// which is what the matrix-core weight gradient multiplies), and code = rint(x / step) has no division error: max error
+// step/2 <= max|x|/127.  e = 255 marks a block that holds an infinity or a NaN: all of it reads back as NaN.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace act8 {
+
+constexpr int BLK = 32;
+
+// exponent byte from the bits of max|x| (an unsigned max over abs bits orders finite < inf < NaN)
+__device__ __forceinline__ int exp_of(unsigned amax_bits) {
+    const int q = (int)(amax_bits >> 23);
+    if (q == 0) return 0;  // zero or subnormal: step 2^-132
+    if (q == 255) return 255;
+    return q - 1 + ((amax_bits & 0x7fffffu) > 0x7e0000u ? 1 : 0);  // mantissa > 127/64: one power more
+}
+__device__ __forceinline__ float code_of(float x, int e) { return e == 255 ? 0.f : rintf(ldexpf(x, 132 - e)); }
+__device__ __forceinline__ float value_of(float code, int e) {
+    return e == 255 ? __builtin_nanf("") : ldexpf(code, e - 132);
+}
+__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// the four codes of a packed word
+__device__ __forceinline__ float code_at(uint32_t w, int k) { return (float)(int8_t)(w >> (8 * k)); }
+
+// max over the L lanes (8 or 32, aligned) that hold one block
+template <int L>
+__device__ __forceinline__ unsigned block_max(unsigned m) {
+#pragma unroll
+    for (int s = 1; s < L; s <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, s));
+    return m;
+}
+
+}  // namespace act8

@@ -278,6 +278,8 @@ class FlatBuffers:
 
     def sync(self):
         ents = self._entries()
+        if not ents:  # a discriminator with group or instance norm has none
+            return None
         if self.flat is None or len(ents) != len(self._ptrs) or \
                 any(b.data_ptr() != ptr for (_, _, b), ptr in zip(ents, self._ptrs)):
             flat = torch.cat([b.detach().reshape(-1) for _, _, b in ents])
@@ -295,7 +297,9 @@ def _broadcast_buffers(module, flat=None):
     if _world() == 1:
         return
     if flat is not None:
-        collective(dist.broadcast, flat.sync(), 0)
+        t = flat.sync()
+        if t is not None:
+            collective(dist.broadcast, t, 0)
         return
     for b in module.buffers():
         collective(dist.broadcast, b, 0)

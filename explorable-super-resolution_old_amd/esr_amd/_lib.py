@@ -8,7 +8,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('ESR_AMD_LIB', os.path.join(_HERE, 'libesr_amd.so'))
-ABI_VERSION = 23
+ABI_VERSION = 24
 
 c_int = ctypes.c_int32
 c_float = ctypes.c_float
@@ -119,6 +119,20 @@ _SIGNATURES = {
                                ctypes.POINTER(c_int), c_int],
     'esr_dconv_wgrad': [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,
                         c_int, c_int, ctypes.POINTER(c_int), ctypes.POINTER(c_int), c_int, c_void_p, c_int, c_void_p],
+    'esr_act8_pack': [c_void_p, ctypes.c_int64, c_int, c_void_p, c_void_p, c_void_p],
+    'esr_act8_unpack': [c_void_p, c_void_p, ctypes.c_int64, c_int, c_void_p, c_void_p],
+    'esr_dconv_wgrad_act8_workspace_bytes': [ctypes.c_int64] + [c_int] * 9,
+    'esr_dconv_wgrad_act8': [c_void_p, c_void_p, ctypes.c_int64, c_int, c_int, c_int, c_void_p, c_int, c_int, c_int,
+                             c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
+    'esr_gn_workspace_bytes': [ctypes.c_int64, ctypes.c_int64, c_int, c_int],
+    'esr_gn_lrelu_fwd': [c_void_p, ctypes.c_int64, ctypes.c_int64, c_int, c_int, c_void_p, c_void_p, c_float, c_float,
+                         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    'esr_gn_lrelu_bwd': [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.c_int64, ctypes.c_int64, c_int, c_int,
+                         c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                         c_void_p],
+    'esr_gn_lrelu_bwd2': [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, ctypes.c_int64,
+                          ctypes.c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p,
+                          c_void_p, c_void_p, c_void_p, c_void_p],
     'esr_timer_create': [c_int],
     'esr_timer_elapsed': [c_void_p, c_fp],
     'esr_timer_destroy': [c_void_p],
@@ -128,7 +142,8 @@ _SIGNATURES = {
     'esr_op_size': [],
     'esr_abi_version': [],
 }
-_RESTYPES = {'esr_timer_create': c_void_p, 'esr_timer_destroy': None, 'esr_bn_workspace_floats': ctypes.c_int64}
+_RESTYPES = {'esr_timer_create': c_void_p, 'esr_timer_destroy': None, 'esr_bn_workspace_floats': ctypes.c_int64,
+             'esr_gn_workspace_bytes': ctypes.c_int64, 'esr_dconv_wgrad_act8_workspace_bytes': ctypes.c_int64}
 EXPORTED = tuple(_SIGNATURES)
 
 # Extra entry points of the ABLATION library (csrc/esr_ablation.h; `make -C .../csrc exp` -> exp_lib/libesr_exp.so):

@@ -22,6 +22,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
+from . import act8
 
 MAX_TAPS = 64
 # Precision of the discriminator convolutions (forward, data and weight gradients): 'x3' = split-f16 operands (hi, lo)
@@ -273,6 +274,37 @@ def conv_wgrad(x, gy, k, s, p, prec=None):
     return red.view(k, k, cin_pad, cout_pad)[:, :, :Ci, :Co].permute(3, 2, 0, 1).contiguous()
 
 
+def conv_wgrad_act8(x8, gy, k, s, p):
+    """conv_wgrad from an input kept in 8 bits: x8 = act8.Act8 of the NHWC input, gy NHWC [B][Ho][Wo][Co] fp32; exact
+    products of the codes' values with gy to fp32 accuracy (csrc/esr_wgrad8.hip)."""
+    act8.check_dev('dconv', gy)
+    if gy.device != x8.codes.device:
+        raise RuntimeError('conv_wgrad_act8: the input is on %s, the gradient on %s' % (x8.codes.device, gy.device))
+    if len(x8.shape) != 4 or gy.dim() != 4:
+        raise ValueError('conv_wgrad_act8: NHWC tensors, got %s and %s' % (tuple(x8.shape), tuple(gy.shape)))
+    B, H, W, Ci = x8.shape
+    Co = gy.shape[3]
+    if not (1 <= k and k * k <= MAX_TAPS and s >= 1 and p >= 0) or min(H, W) + 2 * p < k or \
+            tuple(gy.shape[:3]) != (B, out_size(H, k, s, p), out_size(W, k, s, p)):
+        raise ValueError('conv_wgrad_act8: kernel %d, stride %d, padding %d does not take %s to %s'
+                         % (k, s, p, tuple(x8.shape), tuple(gy.shape)))
+    if B == 0:
+        return gy.new_zeros(Co, Ci, k, k)
+    gy = gy.contiguous()
+    lib = _lib.load()
+    geom = (k, s, p)
+    n = int(lib.esr_dconv_wgrad_act8_workspace_bytes(B, H, W, Ci, gy.shape[1], gy.shape[2], Co, *geom))
+    if n < 0:
+        raise RuntimeError('esr_dconv_wgrad_act8_workspace_bytes failed with esr_status %d' % n)
+    gw = torch.empty(Co, Ci, k, k, device=gy.device, dtype=torch.float32)
+    ws = torch.empty(n, device=gy.device, dtype=torch.uint8)
+    with torch.cuda.device(gy.device):
+        _lib.check(lib.esr_dconv_wgrad_act8(x8.codes.data_ptr(), x8.exps.data_ptr(), B, H, W, Ci, gy.data_ptr(),
+                                            gy.shape[1], gy.shape[2], Co, *geom, gw.data_ptr(), ws.data_ptr(),
+                                            _stream(gy)), 'esr_dconv_wgrad_act8')
+    return gw
+
+
 def colsum(t):
     """Σ over every dimension but the last of a contiguous float tensor (esr_colsum: float64 partial sums in fixed
     order, one pass; PyTorch's sum over (0, 1, 2) of an NHWC tensor ran at ~0.2 TB/s)."""
@@ -285,6 +317,12 @@ def colsum(t):
     ws = torch.empty(int(lib.esr_bn_workspace_floats(P, C)), device=t.device, dtype=torch.float32)
     _lib.check(lib.esr_colsum(t.data_ptr(), P, C, out.data_ptr(), ws.data_ptr(), _stream(t)), 'esr_colsum')
     return out
+
+
+def _bias_grad(gy):
+    if torch.is_grad_enabled() or not COLSUM:  # create_graph: a differentiable sum
+        return gy.sum((0, 1, 2), dtype=torch.float64).float() if BIAS_F64 else gy.sum((0, 1, 2))
+    return colsum(gy)
 
 
 # The precision of a conv is fixed when its forward runs (the module default, or the layer's own
@@ -305,12 +343,7 @@ class DConvFn(torch.autograd.Function):
         gy = gy.contiguous()
         gx = DgradFn.apply(gy, w, k, s, p, x.shape[1], x.shape[2], prec) if ctx.needs_input_grad[0] else None
         gw = WgradFn.apply(x, gy, k, s, p, prec) if ctx.needs_input_grad[1] else None
-        gb = None
-        if ctx.has_bias and ctx.needs_input_grad[2]:
-            if torch.is_grad_enabled() or not COLSUM:  # create_graph: a differentiable sum
-                gb = gy.sum((0, 1, 2), dtype=torch.float64).float() if BIAS_F64 else gy.sum((0, 1, 2))
-            else:
-                gb = colsum(gy)
+        gb = _bias_grad(gy) if ctx.has_bias and ctx.needs_input_grad[2] else None
         return gx, gw, gb, None, None, None, None
 
 
@@ -346,6 +379,49 @@ class WgradFn(torch.autograd.Function):
         g_x = DgradFn.apply(gy, ggw, k, s, p, x.shape[1], x.shape[2], prec) if ctx.needs_input_grad[0] else None
         g_gy = DConvFn.apply(x, ggw, None, k, s, p, prec) if ctx.needs_input_grad[1] else None
         return g_x, g_gy, None, None, None, None
+
+
+class DConvAct8Fn(torch.autograd.Function):
+    """DConvFn that keeps x for the weight gradient in 8 bits: `carrier` = act8.Carrier of x, (codes, exps) = x's
+    blocks.  Forward and data gradient are DConvFn's; the weight gradient is that of the codes' values."""
+
+    @staticmethod
+    def forward(ctx, x, carrier, codes, exps, w, b, k, s, p, prec=None):
+        prec = prec or PRECISION
+        ctx.save_for_backward(carrier, codes, exps, w)
+        ctx.geom = (k, s, p, prec)
+        ctx.has_bias = b is not None
+        return conv_forward(x, w, b, k, s, p, prec)
+
+    @staticmethod
+    def backward(ctx, gy):
+        carrier, codes, exps, w = ctx.saved_tensors
+        k, s, p, prec = ctx.geom
+        gy = gy.contiguous()
+        need = ctx.needs_input_grad
+        gx = DgradFn.apply(gy, w, k, s, p, carrier.shape[1], carrier.shape[2], prec) if need[0] else None
+        gw = WgradAct8Fn.apply(carrier, gy, codes, exps, k, s, p, prec) if need[4] else None
+        gb = _bias_grad(gy) if ctx.has_bias and need[5] else None
+        return gx, None, None, None, gw, gb, None, None, None, None
+
+
+class WgradAct8Fn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, carrier, gy, codes, exps, k, s, p, prec=None):
+        ctx.save_for_backward(carrier, gy, codes, exps)
+        ctx.geom = (k, s, p, prec)
+        return conv_wgrad_act8(act8.Act8(codes, exps), gy, k, s, p)
+
+    @staticmethod
+    def backward(ctx, ggw):
+        carrier, gy, codes, exps = ctx.saved_tensors
+        k, s, p, prec = ctx.geom
+        ggw = ggw.contiguous()
+        g_x = DgradFn.apply(gy, ggw, k, s, p, carrier.shape[1], carrier.shape[2], prec) \
+            if ctx.needs_input_grad[0] else None
+        g_gy = DConvFn.apply(act8.Act8(codes, exps).unpack(), ggw, None, k, s, p, prec) \
+            if ctx.needs_input_grad[1] else None
+        return g_x, g_gy, None, None, None, None, None, None
 
 
 class _ToNHWC(torch.autograd.Function):
@@ -449,22 +525,34 @@ def _df_bwd(xh, gy, mask, slope, w, need_x, need_w):
     return gx, gwb
 
 
+def _df_mask(y, y8):
+    """The layer's output, or its 8-bit values (their y > 0 is the output's) where it was kept so."""
+    return y if y8 is None else act8.Act8(*y8).unpack()
+
+
 class _DFirstFn(torch.autograd.Function):
-    """y = LeakyReLU(conv3x3(x, w) + b) on NHWC tensors (3 -> 64 channels); backward: _DFirstBwdFn."""
+    """y = LeakyReLU(conv3x3(x, w) + b) on NHWC tensors (3 -> 64 channels); backward: _DFirstBwdFn.  keep8: y, whose sign
+    is the backward's mask, is kept in 8 bits, and the result is (y, codes, exps)."""
 
     @staticmethod
-    def forward(ctx, xh, w, b, slope):
+    def forward(ctx, xh, w, b, slope, keep8=False):
         y = _df_fwd(xh, w, b, slope, _DF_LRELU)
-        ctx.save_for_backward(xh, w, y)
-        ctx.slope = slope
-        return y
+        ctx.slope, ctx.keep8 = slope, keep8
+        if not keep8:
+            ctx.save_for_backward(xh, w, y)
+            return y
+        y8 = act8.pack(y)
+        ctx.save_for_backward(xh, w, y8.codes, y8.exps)
+        ctx.mark_non_differentiable(y8.codes, y8.exps)
+        return y, y8.codes, y8.exps
 
     @staticmethod
-    def backward(ctx, gy):
-        xh, w, y = ctx.saved_tensors
+    def backward(ctx, gy, *_unused):
+        xh, w, *y = ctx.saved_tensors
+        y, y8 = (None, tuple(y)) if ctx.keep8 else (y[0], None)
         nx, nw, nb = ctx.needs_input_grad[:3]
-        gx, gw, gb = _DFirstBwdFn.apply(xh, gy.contiguous(), y, w, ctx.slope, nx, nw or nb)
-        return gx if nx else None, gw if nw else None, gb if nb else None, None
+        gx, gw, gb = _DFirstBwdFn.apply(xh, gy.contiguous(), y, w, ctx.slope, nx, nw or nb, y8)
+        return gx if nx else None, gw if nw else None, gb if nb else None, None, None
 
 
 class _DFirstBwdFn(torch.autograd.Function):
@@ -472,12 +560,12 @@ class _DFirstBwdFn(torch.autograd.Function):
     WGAN-GP double backward, loss.py:244-263): with ggx, ggw, ggb the gradients of the three outputs,
         d/dgy = lrelu'(y) · (conv(ggx; w) + conv(x; ggw) + ggb)      (esr_dfirst_fwd, masked)
         d/dw  = wgrad(ggx, g')     d/dx = dgrad(g'; ggw)             (esr_dfirst_bwd)
-    and nothing through y (the mask is piecewise constant)."""
+    and nothing through y (the mask is piecewise constant).  y8: (codes, exps) of y in y's place."""
 
     @staticmethod
-    def forward(ctx, xh, gy, y, w, slope, need_x, need_w):
-        gx, gwb = _df_bwd(xh, gy, y, slope, w, need_x, need_w)
-        ctx.save_for_backward(xh, gy, y, w)
+    def forward(ctx, xh, gy, y, w, slope, need_x, need_w, y8=None):
+        gx, gwb = _df_bwd(xh, gy, _df_mask(y, y8), slope, w, need_x, need_w)
+        ctx.save_for_backward(xh, gy, y, w, *(y8 or ()))
         ctx.slope, ctx.need = slope, (need_x, need_w)
         ctx.set_materialize_grads(False)
         e = gy.new_zeros(0)
@@ -488,7 +576,10 @@ class _DFirstBwdFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, ggx, ggw, ggb):
-        xh, gy, y, w = ctx.saved_tensors
+        xh, gy, y, w, *y8 = ctx.saved_tensors
+        if ggx is None and ggw is None and ggb is None:
+            return (None,) * 8
+        y = _df_mask(y, y8 or None)
         need_x, need_w = ctx.need
         ggx = ggx if need_x and ggx is not None else None
         ggw = ggw if need_w and ggw is not None else None
@@ -512,7 +603,7 @@ class _DFirstBwdFn(torch.autograd.Function):
             g_w = _df_bwd(ggx.contiguous(), gy, y, slope, w, False, True)[1][:64 * 27].view(64, 3, 3, 3)
         if ctx.needs_input_grad[0] and ggw is not None:
             g_x = _df_bwd(None, gy, y, slope, ggw.contiguous(), True, False)[0]
-        return g_x, g_gy, None, g_w, None, None, None
+        return g_x, g_gy, None, g_w, None, None, None, None
 
 
 def dfirst_ok(conv):
@@ -524,12 +615,21 @@ def dfirst_ok(conv):
 def dfirst_lrelu(x, conv, slope):
     """LeakyReLU(slope)(conv(x)) for a HipConv2d passing dfirst_ok, on the fused kernels: NCHW in (any memory format),
     NCHW with channels-last storage out, differentiable twice (the WGAN-GP penalty)."""
+    return dfirst_lrelu8(x, conv, slope)[0]
+
+
+def dfirst_lrelu8(x, conv, slope):
+    """(dfirst_lrelu, its 8-bit blocks where conv.act_checkpoint keeps the output so, for the next convolution to keep as
+    its input; else None)."""
     _check_dev(x)
     if x.is_contiguous(memory_format=torch.channels_last):
         xh = x.permute(0, 2, 3, 1)
     else:
         xh = _ToNHWC.apply(x)
-    return _DFirstFn.apply(xh, conv.weight, conv.bias, float(slope)).permute(0, 3, 1, 2)
+    if conv.keeps8():
+        y, *y8 = _DFirstFn.apply(xh, conv.weight, conv.bias, float(slope), True)
+        return y.permute(0, 3, 1, 2), act8.Act8(*y8)
+    return _DFirstFn.apply(xh, conv.weight, conv.bias, float(slope)).permute(0, 3, 1, 2), None
 
 
 class HipConv2d(nn.Conv2d):
@@ -548,8 +648,14 @@ class HipConv2d(nn.Conv2d):
         # one 32-wide K step instead of one (mostly zero) K step per tap
         self._im2col = s[0] == 1 and self.in_channels * k[0] * k[1] <= 32 and self.in_channels < 8
         self.esr_precision = None  # this layer's precision ('x3' / 'x6' / 'f32'); None = the module default
+        self.act_checkpoint = None  # 'int8': the input is kept for the weight gradient in 8 bits (act8.py)
 
-    def forward(self, x):
+    def keeps8(self):
+        """Whether a forward now keeps its input (the fused first block: its output) in 8 bits."""
+        return bool(act8.check_mode(self.act_checkpoint)) and torch.is_grad_enabled() and self.weight.requires_grad
+
+    def forward(self, x, x8=None):
+        """x8: the input's 8-bit blocks (NHWC), where the caller has them already; used only if the layer keeps them."""
         _check_dev(x)
         if x.is_contiguous(memory_format=torch.channels_last):
             xh = x.permute(0, 2, 3, 1)  # a view: NHWC storage already
@@ -562,6 +668,13 @@ class HipConv2d(nn.Conv2d):
             cols = _Im2ColFn.apply(xh, k, p)  # channel (ky*k + kx)*C + c
             w1 = F.pad(self.weight.permute(0, 2, 3, 1).reshape(self.out_channels, k * k * C), (0, 32 - k * k * C))
             y = DConvFn.apply(cols, w1.view(self.out_channels, 32, 1, 1), self.bias, 1, 1, 0, self.esr_precision)
+        elif self.keeps8():
+            if x8 is None:
+                x8 = act8.pack(xh)
+            elif tuple(x8.shape) != tuple(xh.shape) or x8.codes.device != xh.device:
+                raise ValueError('HipConv2d: input %s, its 8-bit blocks %s' % (tuple(xh.shape), tuple(x8.shape)))
+            y = DConvAct8Fn.apply(xh, act8.Carrier.apply(xh), x8.codes, x8.exps, self.weight, self.bias, k,
+                                  self.stride[0], p, self.esr_precision)
         else:
             y = DConvFn.apply(xh, self.weight, self.bias, k, self.stride[0], p, self.esr_precision)
         return y.permute(0, 3, 1, 2)

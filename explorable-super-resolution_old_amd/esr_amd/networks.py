@@ -74,7 +74,8 @@ def init_weights(net, init_type='kaiming', scale=1, std=0.02):
 
 def define_D(opt, CEM=None):
     """networks.py:105-127.  The shipped `discriminator_vgg_128` + `n_layers` combination builds
-    Discriminator_VGG_128_(nb=n_layers) (the reference's define_G passes nb= to the class without it: TypeError)."""
+    Discriminator_VGG_128_(nb=n_layers) (the reference's define_G passes nb= to the class without it: TypeError).
+    network_D also takes norm_type 'group' (norm_groups, default 32) or 'instance', and act_checkpoint 'int8'."""
     from .discriminator import Discriminator_VGG_128_
     gpu_ids = opt['gpu_ids']
     opt_net = opt['network_D']
@@ -83,7 +84,7 @@ def define_D(opt, CEM=None):
     patch = opt['datasets']['train']['patch_size']
     if CEM is not None:
         patch -= 2 * int(CEM.invalidity_margins_HR)
-    kwargs = {'num_2_strides': opt_net['num_2_strides']} if 'num_2_strides' in opt_net else {}
+    kwargs = {k: opt_net[k] for k in ('num_2_strides', 'norm_groups', 'act_checkpoint') if k in opt_net}
     netD = Discriminator_VGG_128_(in_nc=opt_net['in_nc'], base_nf=opt_net['nf'], norm_type=opt_net['norm_type'],
                                   act_type=opt_net['act_type'], mode=opt_net['mode'], input_patch_size=patch,
                                   nb=opt_net['n_layers'], **kwargs)

@@ -460,6 +460,46 @@ int esr_bn_lrelu_bwd2(const float *x, const float *gy, const float *u, const flo
                       int32_t C, const float *gamma, const float *beta, const float *mu, const float *rs, float slope,
                       const float *sums2, float *g_x, float *g_gy, float *g_gamma, float *ws, esr_stream_t stream);
 
+/* ---- activations kept in 8 bits (esr_act8.hip, esr_wgrad8.hip) ------------------------------------------------------
+ * What the discriminator's blocks keep of an activation x [P][C] (P pixels, channels last) from the forward to the
+ * backward pass: codes int8 [P][C] and one exponent byte per 32 channels of a pixel, exps [P][ceil(C / 32)]; the value
+ * of a code is code · 2^(e − 132), e the smallest with 127 · 2^(e − 132) >= the block's max |x| (e = 255: the block
+ * holds an infinity or a NaN and reads back as NaN).  Error <= half a step <= max|x|/127; x > 0 is kept exactly (a
+ * positive value never takes code 0).  C need not be a multiple of 32 or of 4.
+ * esr_dconv_wgrad_act8: the weight gradient of conv2d(x, w, stride s, zero padding pad) from x's blocks:
+ *   gw[co][ci][ky][kx] = sum over b, Y, X of x[b, s*Y + ky - pad, s*X + kx - pad, ci] * dy[b, Y, X, co]
+ * x [B][Hs][Ws][cin], dy [B][MH][MW][cout] fp32, MH = (Hs + 2·pad − k) / s + 1 (likewise MW), k <= 8, gw in torch's
+ * layout; ws = esr_dconv_wgrad_act8_workspace_bytes(...) bytes (ESR_EINVAL on bad arguments).  Deterministic. */
+int esr_act8_pack(const float *x, int64_t P, int32_t C, int8_t *codes, uint8_t *exps, esr_stream_t stream);
+int esr_act8_unpack(const int8_t *codes, const uint8_t *exps, int64_t P, int32_t C, float *x, esr_stream_t stream);
+int64_t esr_dconv_wgrad_act8_workspace_bytes(int64_t B, int32_t Hs, int32_t Ws, int32_t cin, int32_t MH, int32_t MW,
+                                             int32_t cout, int32_t k, int32_t s, int32_t pad);
+int esr_dconv_wgrad_act8(const int8_t *codes, const uint8_t *exps, int64_t B, int32_t Hs, int32_t Ws, int32_t cin,
+                         const float *dy, int32_t MH, int32_t MW, int32_t cout, int32_t k, int32_t s, int32_t pad,
+                         float *gw, void *ws, esr_stream_t stream);
+
+/* ---- GroupNorm + LeakyReLU, channels last (esr_gn.hip) -------------------------------------------------------------
+ * x, y, gy, ... [N][HW][C] fp32; G groups of C/G channels; gamma, beta [C] or NULL (1, 0; G = C without them is
+ * instance norm).  y = lrelu_slope(γ·(x − μ)·r + β), r = 1/sqrt(v + eps) over each (sample, group).
+ * esr_gn_lrelu_fwd writes y and stat [N][G][2] (μ and r, float64) and, where codes / exps are given, x in 8-bit
+ *   blocks (above) whose pre-activations keep the sign x's have (a code moves one step where rounding would change it).
+ * esr_gn_lrelu_bwd: gx (may be NULL), g_gamma, g_beta (each may be NULL) for upstream gy, and sums [N][2][C] (float64:
+ *   Σ gz, Σ gz·x̂ per sample and channel).  The input is x, or codes / exps with x NULL.
+ * esr_gn_lrelu_bwd2: the backward of (x, γ, gy) -> (gx, dγ, dβ) (the WGAN-GP double backward, loss.py:244-263) for
+ *   upstream u, gg_gamma, gg_beta (each may be NULL = 0) with the sums of esr_gn_lrelu_bwd: g_x, g_gy and g_gamma (may
+ *   be NULL).  ws = esr_gn_workspace_bytes(N, HW, C, G) bytes (ESR_EINVAL on bad arguments).  Deterministic. */
+int64_t esr_gn_workspace_bytes(int64_t N, int64_t HW, int32_t C, int32_t G);
+int esr_gn_lrelu_fwd(const float *x, int64_t N, int64_t HW, int32_t C, int32_t G, const float *gamma, const float *beta,
+                     float eps, float slope, float *y, double *stat, int8_t *codes, uint8_t *exps, void *ws,
+                     esr_stream_t stream);
+int esr_gn_lrelu_bwd(const float *x, const int8_t *codes, const uint8_t *exps, const float *gy, int64_t N, int64_t HW,
+                     int32_t C, int32_t G, const float *gamma, const float *beta, const double *stat, float slope,
+                     float *gx, float *g_gamma, float *g_beta, double *sums, void *ws, esr_stream_t stream);
+int esr_gn_lrelu_bwd2(const float *x, const int8_t *codes, const uint8_t *exps, const float *gy, const float *u,
+                      const float *gg_gamma, const float *gg_beta, int64_t N, int64_t HW, int32_t C, int32_t G,
+                      const float *gamma, const float *beta, const double *stat, float slope, const double *sums,
+                      float *g_x, float *g_gy, float *g_gamma, void *ws, esr_stream_t stream);
+
 /* Library / ABI version (bumped on any signature change). */
 int esr_abi_version(void);
 
