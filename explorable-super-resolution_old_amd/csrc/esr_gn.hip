@@ -21,12 +21,17 @@
 #include "esr_act8.h"
 #include "esr_amd.h"
 #include "esr_knobs.h"
+#include <initializer_list>
 
 namespace {
 
 constexpr int NT = 256;
-constexpr int MAXS = 64;  // row splits of a sample in a reduction
+constexpr int MAXS = 256;   // row splits of a sample in a reduction
+constexpr int UN = 4;       // rows of a thread in flight
 
+// A thread holds V consecutive channels (V = 4: 16-byte accesses; V = 1 where C or a base is not a multiple of 4 values)
+// and walks rows; the 32 / V lanes of an 8-bit block sit side by side, a row takes `lanes` threads (its last block padded
+// to 32 channels) and a workgroup `rpi` rows at a time.  Rows wider than a workgroup are cut over blockIdx.z.
 struct GnP {
     const float *x;              // [N][HW][C], or null: codes / exps
     const int8_t *codes;
@@ -36,298 +41,492 @@ struct GnP {
     const float *gga, *ggb;      // [C] upstream of dγ, dβ, or null
     const double *stat;          // [N][G][2]: μ and r
     const double *grp;           // [N][G][8] per-group coefficients of the pass
+    const double *sums, *sums_u; // [N][2][C]: s1, s2; [N][3][C]: Σu, Σu·x̂, Σu·gz
     long long HW;
-    int N, C, G, Cg, splits;
+    int N, C, G, Cg, nb, lanes, rpi, chunks, splits, blocks;
     float slope, eps;
 };
 
-__device__ __forceinline__ float load_x(const GnP &p, long long row, int c) {
-    if (p.x) return p.x[row * p.C + c];
-    const int nb = (p.C + act8::BLK - 1) / act8::BLK;
-    return act8::value_of((float)p.codes[row * p.C + c], p.exps[row * nb + c / act8::BLK]);
-}
 // x̂ and z of one value, by the same operations everywhere.  (x − μ)·r rather than x·r − μ·r: the values of a constant
 // group are their mean exactly, and their z is β.
 __device__ __forceinline__ double xhat(double x, double r, double mu) { return (x - mu) * r; }
 __device__ __forceinline__ double preact(double xh, double gamma, double beta) { return fma(gamma, xh, beta); }
 
-// per-(sample, split, channel) sums: MODE 0: Σd, Σd² (d = x − the group's first value); 1: Σgz, Σgz·x̂; 2: Σu, Σu·x̂, Σu·gz
-template <int MODE>
-__global__ __launch_bounds__(NT) void gn_colsum(GnP p, double *partial) {
+template <int V>
+__device__ __forceinline__ void load_f(const float *src, long long i, float *v) {
+    if constexpr (V == 4) {
+        const float4 t = *reinterpret_cast<const float4 *>(src + i);
+        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+    } else {
+        v[0] = src[i];
+    }
+}
+template <int V>
+__device__ __forceinline__ void store_f(float *dst, long long i, const float *v) {
+    if constexpr (V == 4) *reinterpret_cast<float4 *>(dst + i) = make_float4(v[0], v[1], v[2], v[3]);
+    else dst[i] = v[0];
+}
+// a row's raw input (values, or a word of codes and its exponent byte), loaded ahead of its use
+template <int V, bool Q8>
+struct Raw {
+    float v[V];
+    uint32_t w;
+    int e;
+    __device__ __forceinline__ void load(const GnP &p, long long row, int c) {
+        if constexpr (Q8) {
+            if constexpr (V == 4) w = *reinterpret_cast<const uint32_t *>(p.codes + row * p.C + c);
+            else w = (uint8_t)p.codes[row * p.C + c];
+            e = p.exps[row * p.nb + c / act8::BLK];
+        } else {
+            load_f<V>(p.x, row * p.C + c, v);
+        }
+    }
+    __device__ __forceinline__ float at(int k) const {
+        if constexpr (Q8) return act8::value_of(act8::code_at(w, k), e);
+        else return v[k];
+    }
+};
+// per-channel constants of a thread
+template <int V>
+struct Chan {
+    double mu[V], r[V], ga[V], be[V];
+    __device__ __forceinline__ void load(const GnP &p, int n, int c) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const long long g = (long long)n * p.G + (c + k) / p.Cg;
+            mu[k] = p.stat[2 * g];
+            r[k] = p.stat[2 * g + 1];
+            ga[k] = p.gamma ? (double)p.gamma[c + k] : 1.0;
+            be[k] = p.beta ? (double)p.beta[c + k] : 0.0;
+        }
+    }
+};
+
+// partial[n][split][k][c]: MODE 0: Σd, Σd² (d = x − the group's first value); 1: Σgz, Σgz·x̂; 2: Σu, Σu·x̂, Σu·gz
+template <int MODE, int V, bool Q8>
+__global__ __launch_bounds__(NT) void gn_sums(GnP p, double *partial) {
     constexpr int K = MODE == 2 ? 3 : 2;
-    const int n = blockIdx.y, sp = blockIdx.x;
+    __shared__ double red[K * V][NT];
+    const int tid = threadIdx.x, lane = tid % p.lanes, ph = tid / p.lanes, n = blockIdx.y, sp = blockIdx.x;
+    const int c = ((int)blockIdx.z * NT + lane) * V;
     const long long r0 = p.HW * sp / p.splits, r1 = p.HW * (sp + 1) / p.splits;
-    __shared__ double red[K][NT];
-    const int rpi = p.C <= NT ? NT / p.C : 1;
-    for (int cb = 0; cb < p.C; cb += NT) {
-        const int c = p.C <= NT ? (int)threadIdx.x % p.C : cb + (int)threadIdx.x;
-        const int ph = p.C <= NT ? (int)threadIdx.x / p.C : 0;
-        const bool act = c < p.C && ph < rpi;
-        double s[K] = {};
-        if (act) {
-            const int g = c / p.Cg;
-            const double pivot = MODE == 0 ? (double)p.x[(long long)n * p.HW * p.C + g * p.Cg] : 0.0;
-            const double mu = MODE ? p.stat[((long long)n * p.G + g) * 2] : 0.0;
-            const double r = MODE ? p.stat[((long long)n * p.G + g) * 2 + 1] : 0.0;
-            const double ga = p.gamma ? p.gamma[c] : 1.0, be = p.beta ? p.beta[c] : 0.0;
-            for (long long q = r0 + ph; q < r1; q += rpi) {
-                const long long row = (long long)n * p.HW + q, i = row * p.C + c;
-                const float x = load_x(p, row, c);
-                if (MODE == 0) {
-                    const double d = (double)x - pivot;
-                    s[0] += d;
-                    s[1] = fma(d, d, s[1]);
-                } else {
-                    const double xh = xhat(x, r, mu);
-                    const double gz = (double)(p.gy[i] * (preact(xh, ga, be) > 0.0 ? 1.f : p.slope));
-                    if (MODE == 1) {
-                        s[0] += gz;
-                        s[1] = fma(gz, xh, s[1]);
+    double s[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) s[k][v] = 0.0;
+    if (ph < p.rpi && c < p.C) {
+        Chan<V> ch;
+        double pivot[V];
+        if constexpr (MODE == 0) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) pivot[v] = p.x[(long long)n * p.HW * p.C + (c + v) / p.Cg * p.Cg];
+        } else {
+            ch.load(p, n, c);
+        }
+        for (long long q = r0 + ph; q < r1; q += UN * p.rpi) {
+            Raw<V, Q8> raw[UN];
+            float gy[UN][V], u[UN][V];
+#pragma unroll
+            for (int j = 0; j < UN; ++j) {  // rows past the end load the last one and are not added
+                const long long row = (long long)n * p.HW + min(q + j * p.rpi, r1 - 1);
+                raw[j].load(p, row, c);
+                if constexpr (MODE >= 1) load_f<V>(p.gy, row * p.C + c, gy[j]);
+                if constexpr (MODE == 2) load_f<V>(p.u, row * p.C + c, u[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < UN; ++j) {
+                if (q + j * p.rpi >= r1) break;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const double x = raw[j].at(v);
+                    if constexpr (MODE == 0) {
+                        const double d = x - pivot[v];
+                        s[0][v] += d;
+                        s[1][v] = fma(d, d, s[1][v]);
                     } else {
-                        const double u = p.u[i];
-                        s[0] += u;
-                        s[1] = fma(u, xh, s[1]);
-                        s[2] = fma(u, gz, s[2]);
+                        const double xh = xhat(x, ch.r[v], ch.mu[v]);
+                        const double gz = gy[j][v] * (preact(xh, ch.ga[v], ch.be[v]) > 0.0 ? 1.f : p.slope);
+                        if constexpr (MODE == 1) {
+                            s[0][v] += gz;
+                            s[1][v] = fma(gz, xh, s[1][v]);
+                        } else {
+                            s[0][v] += u[j][v];
+                            s[1][v] = fma((double)u[j][v], xh, s[1][v]);
+                            s[K - 1][v] = fma((double)u[j][v], gz, s[K - 1][v]);
+                        }
                     }
                 }
             }
         }
-        for (int k = 0; k < K; ++k) red[k][threadIdx.x] = s[k];
-        __syncthreads();
-        if (ph == 0 && c < p.C)
-            for (int k = 0; k < K; ++k) {
-                double v = red[k][threadIdx.x];
-                for (int q = 1; q < rpi; ++q) v += red[k][q * p.C + threadIdx.x];
-                partial[(((long long)n * p.splits + sp) * K + k) * p.C + c] = v;
-            }
-        __syncthreads();
-        if (p.C <= NT) break;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) red[k * V + v][tid] = s[k][v];
+    __syncthreads();
+    for (int i = tid; i < K * V * p.lanes; i += NT) {  // the rows of a workgroup, in order
+        const int ln = i / V % p.lanes, k = i / V / p.lanes, v = i % V;
+        const int cc = ((int)blockIdx.z * NT + ln) * V + v;
+        if (cc >= p.C) continue;
+        double t = red[k * V + v][ln];
+        for (int q = 1; q < p.rpi; ++q) t += red[k * V + v][q * p.lanes + ln];
+        partial[(((long long)n * p.splits + sp) * K + k) * p.C + cc] = t;
     }
 }
 
-// sums[n][k][c] = Σ over splits, in order
-__global__ void gn_splits(const double *partial, int splits, int KC, double *sums) {
-    const int n = blockIdx.y, i = blockIdx.x * NT + threadIdx.x;
-    if (i >= KC) return;
-    double v = 0.0;
-    for (int s = 0; s < splits; ++s) v += partial[((long long)n * splits + s) * KC + i];
-    sums[(long long)n * KC + i] = v;
-}
-
-// MODE 0: stat (μ, r) of each group; 1: grp = S1/M, S2/M; 2: the seven coefficients of the double backward
+// One workgroup per sample and set of whole groups (32 channels' worth, or one larger group): the splits' sums per
+// channel (sums_out [n][K][C], or null), then each group's: MODE 0: out = μ, r; 1: S1/M, S2/M; 2: the seven coefficients
+// of the double backward (partial null: no upstream of gx).
 template <int MODE>
-__global__ void gn_groups(GnP p, const double *sums, const double *sums_u, double *out) {
-    const int i = blockIdx.x * NT + threadIdx.x;
-    if (i >= p.N * p.G) return;
-    const int n = i / p.G, g = i - n * p.G;
-    const double M = (double)p.HW * p.Cg;
-    const double *s = sums + (long long)n * 2 * p.C;
-    double t0 = 0, t1 = 0, b0 = 0, b1 = 0, U = 0, A = 0, Q = 0;
-    for (int c = g * p.Cg; c < (g + 1) * p.Cg; ++c) {
-        const double ga = MODE && p.gamma ? p.gamma[c] : 1.0;
-        t0 += ga * s[c];
-        t1 += ga * s[p.C + c];
-        if (MODE == 2) {
-            if (p.gga) {
-                b0 += (double)p.gga[c] * s[c];
-                b1 += (double)p.gga[c] * s[p.C + c];
+__global__ __launch_bounds__(NT) void gn_finish(GnP p, const double *partial, double *sums_out, double *out) {
+    constexpr int K = MODE == 2 ? 3 : 2, J = MODE == 2 ? 7 : 2;
+    __shared__ double part[8][K][32], chan[J][33], tot[J][32];
+    const int tid = threadIdx.x, lane = tid & 31, sl = tid >> 5, n = blockIdx.y;
+    const int gpb = p.Cg <= 32 ? 32 / p.Cg : 1, g0 = blockIdx.x * gpb, ng = min(gpb, p.G - g0);
+    const int c1 = (g0 + ng) * p.Cg;
+    for (int i = tid; i < J * 32; i += NT) tot[i / 32][i % 32] = 0.0;
+    for (int c0 = g0 * p.Cg; c0 < c1; c0 += 32) {
+        const int c = c0 + lane;
+        double s[K] = {};
+        if (c < c1 && partial)
+#pragma unroll 4
+            for (int sp = sl; sp < p.splits; sp += 8)
+#pragma unroll
+                for (int k = 0; k < K; ++k) s[k] += partial[(((long long)n * p.splits + sp) * K + k) * p.C + c];
+#pragma unroll
+        for (int k = 0; k < K; ++k) part[sl][k][lane] = s[k];
+        __syncthreads();
+        if (sl == 0) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                s[k] = part[0][k][lane];
+                for (int q = 1; q < 8; ++q) s[k] += part[q][k][lane];
+                if (sums_out && c < c1) sums_out[((long long)n * K + k) * p.C + c] = s[k];
             }
-            if (sums_u) {
-                const double *v = sums_u + (long long)n * 3 * p.C;
-                U += v[c];
-                A += v[p.C + c];
-                Q += ga * v[2 * p.C + c];
+            const double ga = MODE && p.gamma && c < c1 ? (double)p.gamma[c] : 1.0;
+            if constexpr (MODE < 2) {
+                chan[0][lane] = ga * s[0];
+                chan[1][lane] = ga * s[1];
+            } else {
+                const bool in = c < c1;
+                const double s1 = in ? p.sums[(long long)n * 2 * p.C + c] : 0.0;
+                const double s2 = in ? p.sums[((long long)n * 2 + 1) * p.C + c] : 0.0;
+                const double a = in && p.gga ? (double)p.gga[c] : 0.0;
+                chan[0][lane] = ga * s1;
+                chan[1][lane] = ga * s2;
+                chan[2][lane] = s[0];
+                chan[3][lane] = s[1];
+                chan[4][lane] = ga * s[K - 1];
+                chan[5][lane] = p.gga ? a * s1 : 0.0;
+                chan[6][lane] = p.gga ? a * s2 : 0.0;
             }
         }
+        __syncthreads();
+        for (int i = tid; i < J * ng; i += NT) {  // channels of a group, in order
+            const int j = i / ng, g = i - j * ng, a = p.Cg <= 32 ? g * p.Cg : 0;
+            const int b = p.Cg <= 32 ? a + p.Cg : min(32, c1 - c0);
+            double t = tot[j][g];
+            for (int k = a; k < b; ++k) t += chan[j][k];
+            tot[j][g] = t;
+        }
+        __syncthreads();
     }
-    if (MODE == 0) {
-        const double pivot = p.x[(long long)n * p.HW * p.C + g * p.Cg];
-        const double d = t0 / M, var0 = t1 / M - d * d, var = var0 < 0.0 ? 0.0 : var0;  // (a NaN stays one)
-        const double r = 1.0 / sqrt(var + (double)p.eps);
-        out[2 * i] = pivot + d;
-        out[2 * i + 1] = r;
-    } else if (MODE == 1) {
-        out[8 * i] = t0 / M;
-        out[8 * i + 1] = t1 / M;
+    if (tid >= ng) return;
+    const long long i = (long long)n * p.G + g0 + tid;
+    const double M = (double)p.HW * p.Cg, t0 = tot[0][tid] / M, t1 = tot[1][tid] / M;
+    if constexpr (MODE == 0) {
+        const double var0 = t1 - t0 * t0, var = var0 < 0.0 ? 0.0 : var0;  // (a NaN stays one)
+        out[2 * i] = p.x[(long long)n * p.HW * p.C + (g0 + tid) * p.Cg] + t0;
+        out[2 * i + 1] = 1.0 / sqrt(var + (double)p.eps);
+    } else if constexpr (MODE == 1) {
+        out[8 * i] = t0;
+        out[8 * i + 1] = t1;
     } else {
-        const double r = p.stat[2 * i + 1], m1 = t0 / M, m2 = t1 / M, u = U / M, a = A / M;
+        const double r = p.stat[2 * i + 1], u = tot[J - 5][tid] / M, a = tot[J - 4][tid] / M;
         out[8 * i] = u;
         out[8 * i + 1] = a;
-        out[8 * i + 2] = m1;
-        out[8 * i + 3] = m2;
-        out[8 * i + 4] = -r * (m1 * a + u * m2) + b0 / M;
-        out[8 * i + 5] = -2.0 * r * m2 * a + b1 / M;
-        out[8 * i + 6] = (Q / M - m1 * u - m2 * a) * r * r;
+        out[8 * i + 2] = t0;
+        out[8 * i + 3] = t1;
+        out[8 * i + 4] = -r * (t0 * a + u * t1) + tot[J - 2][tid] / M;
+        out[8 * i + 5] = -2.0 * r * t1 * a + tot[J - 1][tid] / M;
+        out[8 * i + 6] = (tot[J - 3][tid] / M - t0 * u - t1 * a) * r * r;
     }
 }
 
-// dβ, dγ from s1, s2 (MODE 1), or g_γ (MODE 2): sums over the samples, in order
-template <int MODE>
-__global__ void gn_params(GnP p, const double *sums, const double *sums_u, float *o1, float *o2) {
-    const int c = blockIdx.x * NT + threadIdx.x;
-    if (c >= p.C) return;
-    double a = 0.0, b = 0.0;
-    for (int n = 0; n < p.N; ++n) {
-        const double *s = sums + (long long)n * 2 * p.C;
-        if (MODE == 1) {
-            a += s[p.C + c];
-            b += s[c];
-        } else if (sums_u) {
-            const long long i = (long long)n * p.G + c / p.Cg;
-            a += p.stat[2 * i + 1] * (sums_u[((long long)n * 3 + 2) * p.C + c] - s[c] * p.grp[8 * i] -
-                                      s[p.C + c] * p.grp[8 * i + 1]);
-        }
-    }
-    if (o1) o1[c] = (float)a;
-    if (MODE == 1 && o2) o2[c] = (float)b;
-}
-
-// MODE 0: y (and x's 8-bit blocks); 1: gx; 2: g_x (o1) and g_gy (o2).  A thread per value, lanes of a 32-channel block
-// together (the last block of a row padded to 32 lanes).
-template <int MODE>
-__global__ __launch_bounds__(NT) void gn_apply(GnP p, float *o1, float *o2, int8_t *codes, uint8_t *exps) {
-    const int nb = (p.C + act8::BLK - 1) / act8::BLK, rl = nb * act8::BLK;
-    const long long q = (long long)blockIdx.x * NT + threadIdx.x, row = q / rl;
-    const int c = (int)(q - row * rl);
-    const bool act = row < p.N * p.HW && c < p.C;
-    float x = 0.f;
-    double r = 0, mu = 0, ga = 1, be = 0, xd = 0, z = 0;
-    long long gi = 0;
-    if (act) {
-        x = load_x(p, row, c);
-        gi = row / p.HW * p.G + c / p.Cg;
-        mu = p.stat[2 * gi];
-        r = p.stat[2 * gi + 1];
-        if (p.gamma) ga = p.gamma[c];
-        if (p.beta) be = p.beta[c];
-        xd = xhat(x, r, mu);
-        z = preact(xd, ga, be);
-    }
-    const long long i = row * p.C + c;
-    if (MODE == 0) {
-        if (act) o1[i] = (float)(z > 0.0 ? z : (double)p.slope * z);
-        if (!codes) return;
-        const int e = act8::exp_of(act8::block_max<32>(act8::abs_bits(x)));
-        if (!act) return;
-        float code = act8::code_of(x, e);
-        if (e != 255) {
-            const float v = act8::value_of(code, e);
-            if ((preact(xhat(v, r, mu), ga, be) > 0.0) != (z > 0.0)) code += v > x ? -1.f : 1.f;
-        }
-        codes[i] = (int8_t)(int)code;
-        if (c % act8::BLK == 0) exps[row * nb + c / act8::BLK] = (uint8_t)e;
-        return;
-    }
+// codes of V values of one row in a block whose lanes call together; pre: z of a value
+template <int V, typename F>
+__device__ __forceinline__ void put_blocks(const GnP &p, const float *v, bool act, long long row, int c, int lane,
+                                           int8_t *codes, uint8_t *exps, F pre) {
+    constexpr int L = act8::BLK / V;
+    unsigned m = 0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) m = max(m, act8::abs_bits(v[k]));
+    const int e = act8::exp_of(act8::block_max<L>(m));
     if (!act) return;
-    const float m = z > 0.0 ? 1.f : p.slope, xh = (float)xd, rf = (float)r, gf = (float)ga;
-    const double *k = p.grp + 8 * gi;
-    const float gz = p.gy[i] * m, h = gf * gz;
-    if (MODE == 1) {
-        o1[i] = rf * (h - (float)k[0] - xh * (float)k[1]);
-        return;
+    uint32_t w = 0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        float code = act8::code_of(v[k], e);
+        if (e != 255) {
+            const float at = act8::value_of(code, e);
+            if (pre(at, k) != pre(v[k], k)) code += at > v[k] ? -1.f : 1.f;
+        }
+        w |= (uint32_t)(uint8_t)(int8_t)(int)code << (8 * k);
     }
-    const float u = p.u ? p.u[i] : 0.f, ua = p.gga ? p.gga[c] : 0.f, ub = p.ggb ? p.ggb[c] : 0.f;
-    o2[i] = m * (gf * rf * (u - (float)k[0] - xh * (float)k[1]) + ua * xh + ub);
-    const float gg = -rf * (h * (float)k[1] + u * (float)k[3]) + ua * gz;
-    o1[i] = rf * (gg - (float)k[4] - xh * (float)k[5]) - (float)k[6] * xh;
+    if constexpr (V == 4) *reinterpret_cast<uint32_t *>(codes + row * p.C + c) = w;
+    else codes[row * p.C + c] = (int8_t)w;
+    if (lane % L == 0) exps[row * p.nb + c / act8::BLK] = (uint8_t)e;
+}
+
+struct GnOut {
+    float *o1, *o2;          // MODE 0: y; 1: gx; 2: g_x, g_gy
+    float *g_gamma, *g_beta; // [C] or null
+    int8_t *codes, *ycodes;  // MODE 0: x's and y's 8-bit blocks, or null
+    uint8_t *exps, *yexps;
+};
+
+// The elementwise pass.  Workgroups go through samples and rows from the last to the first: what the reduction before
+// read last is still in the 256 MB last-level cache.  The first row block of the first sample also sums the parameter
+// gradients over the samples, in order.
+template <int MODE, int V, bool Q8>
+__global__ __launch_bounds__(NT) void gn_apply(GnP p, GnOut o) {
+    constexpr int UA = MODE == 2 ? 2 : UN;
+    const int tid = threadIdx.x, lane = tid % p.lanes, ph = tid / p.lanes;
+    const int n = p.N - 1 - (int)blockIdx.y, b = p.blocks - 1 - (int)blockIdx.x;
+    const int c = ((int)blockIdx.z * NT + lane) * V;
+    const bool act = c < p.C;
+    if (ph >= p.rpi) return;
+    if (MODE && b == 0 && n == 0 && ph == 0 && act) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            double s = 0.0, t = 0.0;
+            for (int i = 0; i < p.N; ++i) {
+                const double *q = p.sums + (long long)i * 2 * p.C + c + v;
+                if constexpr (MODE == 1) {
+                    s += q[p.C];
+                    t += q[0];
+                } else if (p.sums_u) {
+                    const long long g = (long long)i * p.G + (c + v) / p.Cg;
+                    s += p.stat[2 * g + 1] * (p.sums_u[((long long)i * 3 + 2) * p.C + c + v] - q[0] * p.grp[8 * g] -
+                                              q[p.C] * p.grp[8 * g + 1]);
+                }
+            }
+            if (o.g_gamma) o.g_gamma[c + v] = (float)s;
+            if (MODE == 1 && o.g_beta) o.g_beta[c + v] = (float)t;
+        }
+    }
+    Chan<V> ch;
+    float k0[V], k1[V], k3[V], k4[V], k5[V], k6[V], ua[V], ub[V];
+    if (act) {
+        ch.load(p, n, c);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if constexpr (MODE >= 1) {
+                const double *k = p.grp + 8 * ((long long)n * p.G + (c + v) / p.Cg);
+                k0[v] = (float)k[0];
+                k1[v] = (float)k[1];
+                if constexpr (MODE == 2) {
+                    k3[v] = (float)k[3];
+                    k4[v] = (float)k[4];
+                    k5[v] = (float)k[5];
+                    k6[v] = (float)k[6];
+                    ua[v] = p.gga ? p.gga[c + v] : 0.f;
+                    ub[v] = p.ggb ? p.ggb[c + v] : 0.f;
+                }
+            }
+        }
+    }
+    const long long r0 = p.HW * b / p.blocks, r1 = p.HW * (b + 1) / p.blocks;
+    for (long long q = r0 + ph; q < r1; q += UA * p.rpi) {
+        Raw<V, Q8> raw[UA];
+        float gy[UA][V], u[UA][V];
+        if (act) {
+#pragma unroll
+            for (int j = 0; j < UA; ++j) {
+                const long long row = (long long)n * p.HW + min(q + j * p.rpi, r1 - 1);
+                raw[j].load(p, row, c);
+                if constexpr (MODE >= 1) load_f<V>(p.gy, row * p.C + c, gy[j]);
+                if constexpr (MODE == 2) {
+                    if (p.u) load_f<V>(p.u, row * p.C + c, u[j]);
+                    else
+#pragma unroll
+                        for (int v = 0; v < V; ++v) u[j][v] = 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < UA; ++j) {
+            if (q + j * p.rpi >= r1) break;
+            const long long row = (long long)n * p.HW + q + j * p.rpi;
+            float a[V], d[V];
+            if (act) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const double xd = xhat(raw[j].at(v), ch.r[v], ch.mu[v]), z = preact(xd, ch.ga[v], ch.be[v]);
+                    if constexpr (MODE == 0) {
+                        a[v] = (float)(z * (z > 0.0 ? 1.0 : (double)p.slope));
+                    } else {
+                        const float m = z > 0.0 ? 1.f : p.slope, xh = (float)xd, rf = (float)ch.r[v], gf = (float)ch.ga[v];
+                        const float gz = gy[j][v] * m, h = gf * gz;
+                        if constexpr (MODE == 1) {
+                            a[v] = rf * (h - k0[v] - xh * k1[v]);
+                        } else {
+                            const float uu = u[j][v], gg = -rf * (h * k1[v] + uu * k3[v]) + ua[v] * gz;
+                            d[v] = m * (gf * rf * (uu - k0[v] - xh * k1[v]) + ua[v] * xh + ub[v]);
+                            a[v] = rf * (gg - k4[v] - xh * k5[v]) - k6[v] * xh;
+                        }
+                    }
+                }
+                store_f<V>(o.o1, row * p.C + c, a);
+                if constexpr (MODE == 2) store_f<V>(o.o2, row * p.C + c, d);
+            }
+            if constexpr (MODE == 0 && !Q8) {
+                if (o.codes || o.ycodes) {
+                    float t[V];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        t[v] = act ? raw[j].at(v) : 0.f;
+                        a[v] = act ? a[v] : 0.f;
+                    }
+                    if (o.codes)
+                        put_blocks<V>(p, t, act, row, c, lane, o.codes, o.exps, [&](float x, int v) {
+                            return preact(xhat(x, ch.r[v], ch.mu[v]), ch.ga[v], ch.be[v]) > 0.0;
+                        });
+                    if (o.ycodes)
+                        put_blocks<V>(p, a, act, row, c, lane, o.ycodes, o.yexps, [](float y, int) { return y > 0.f; });
+                }
+            }
+        }
+    }
 }
 
 inline int launched() { return hipGetLastError() == hipSuccess ? ESR_OK : ESR_ELAUNCH; }
-inline unsigned blocks_of(long long n) { return (unsigned)((n + NT - 1) / NT); }
 
 inline bool shape_ok(int64_t N, int64_t HW, int32_t C, int32_t G) {
-    if (N <= 0 || HW <= 0 || C <= 0 || G <= 0 || C % G) return false;
+    if (N <= 0 || HW <= 0 || C <= 0 || G <= 0 || C % G || C > (1 << 24)) return false;
     if (N > 65535 || (int64_t)N * G > 0x7fffffffLL) return false;
-    const int64_t rl = (C + 31) / 32 * 32;
-    return HW <= 0x7fffffffLL * NT / rl / N;  // the elementwise grid
-}
-inline int splits_of(int64_t N, int64_t HW) {
-    const int64_t s = HW / 64;
-    return (int)(s < 1 ? 1 : (s > MAXS ? MAXS : s));
+    return HW <= (1LL << 46) / C / N;  // element offsets, with room for the row arithmetic
 }
 inline bool bits_ok(const void *x, const void *codes, const void *exps) {
     return x ? !codes && !exps : codes && exps;  // exactly one form of the input
 }
-
-template <int MODE>
-void colsum(const GnP &p, double *partial, double *sums, hipStream_t st) {
-    constexpr int K = MODE == 2 ? 3 : 2;
-    hipLaunchKernelGGL(gn_colsum<MODE>, dim3(p.splits, p.N), dim3(NT), 0, st, p, partial);
-    hipLaunchKernelGGL(gn_splits, dim3(blocks_of((long long)K * p.C), p.N), dim3(NT), 0, st, partial, p.splits, K * p.C,
-                       sums);
+inline bool aligned(std::initializer_list<const void *> f32, std::initializer_list<const void *> codes) {
+    for (const void *q : f32)
+        if ((uintptr_t)q % 16) return false;
+    for (const void *q : codes)
+        if ((uintptr_t)q % 4) return false;
+    return true;
 }
 
-GnP params(const float *x, const int8_t *codes, const uint8_t *exps, int64_t N, int64_t HW, int32_t C, int32_t G,
-           const float *gamma, const float *beta, float slope) {
+GnP params(int V, int64_t N, int64_t HW, int32_t C, int32_t G, const float *gamma, const float *beta, float slope) {
     GnP p{};
-    p.x = x; p.codes = codes; p.exps = exps; p.gamma = gamma; p.beta = beta;
+    p.gamma = gamma; p.beta = beta;
     p.N = (int)N; p.HW = HW; p.C = C; p.G = G; p.Cg = C / G; p.slope = slope;
-    p.splits = splits_of(N, HW);
+    p.nb = (C + act8::BLK - 1) / act8::BLK;
+    const int lanes = p.nb * (act8::BLK / V);
+    p.chunks = (lanes + NT - 1) / NT;
+    p.lanes = lanes < NT ? lanes : NT;
+    p.rpi = NT / p.lanes;
+    // ~4 workgroups per CU for the sums (each leaves K·C float64 partials), 16 for the elementwise pass, of at least UN
+    // rows per thread
+    const int64_t per = (int64_t)N * p.chunks, rows = (HW + UN * p.rpi - 1) / (UN * p.rpi);
+    auto cut = [&](int64_t want, int64_t most) {
+        int64_t s = (want + per - 1) / per;
+        s = s < rows ? s : rows;
+        return (int)(s < most ? s : most);
+    };
+    p.splits = cut(1024, MAXS);
+    p.blocks = cut(4096, 0x7fffffff);
     return p;
+}
+
+template <int MODE, bool Q8>
+void sums(const GnP &p, int V, double *partial, hipStream_t st) {
+    const dim3 grid(p.splits, p.N, p.chunks);
+    if (V == 4) hipLaunchKernelGGL((gn_sums<MODE, 4, Q8>), grid, dim3(NT), 0, st, p, partial);
+    else hipLaunchKernelGGL((gn_sums<MODE, 1, Q8>), grid, dim3(NT), 0, st, p, partial);
+}
+template <int MODE>
+void finish(const GnP &p, const double *partial, double *sums_out, double *out, hipStream_t st) {
+    const int gpb = p.Cg <= 32 ? 32 / p.Cg : 1;
+    hipLaunchKernelGGL(gn_finish<MODE>, dim3((p.G + gpb - 1) / gpb, p.N), dim3(NT), 0, st, p, partial, sums_out, out);
+}
+template <int MODE, bool Q8>
+void apply(const GnP &p, int V, const GnOut &o, hipStream_t st) {
+    const dim3 grid(p.blocks, p.N, p.chunks);
+    if (V == 4) hipLaunchKernelGGL((gn_apply<MODE, 4, Q8>), grid, dim3(NT), 0, st, p, o);
+    else hipLaunchKernelGGL((gn_apply<MODE, 1, Q8>), grid, dim3(NT), 0, st, p, o);
 }
 
 }  // namespace
 
 extern "C" int64_t esr_gn_workspace_bytes(int64_t N, int64_t HW, int32_t C, int32_t G) {
     if (!shape_ok(N, HW, C, G)) return ESR_EINVAL;
+    const int64_t s1 = params(1, N, HW, C, G, nullptr, nullptr, 0.f).splits;
+    const int64_t s4 = params(4, N, HW, C, G, nullptr, nullptr, 0.f).splits;
     // split sums [N][splits][3][C], sums of u [N][3][C], group coefficients [N][G][8]
-    return 8 * (N * splits_of(N, HW) * 3 * C + N * 3 * C + N * G * 8);
+    return 8 * (N * (s1 > s4 ? s1 : s4) * 3 * C + N * 3 * C + N * G * 8);
 }
 
 extern "C" int esr_gn_lrelu_fwd(const float *x, int64_t N, int64_t HW, int32_t C, int32_t G, const float *gamma,
                                 const float *beta, float eps, float slope, float *y, double *stat, int8_t *codes,
-                                uint8_t *exps, void *ws, esr_stream_t stream) {
-    if (!x || !y || !stat || !ws || !shape_ok(N, HW, C, G) || !(eps >= 0.f) || !codes != !exps) return ESR_EINVAL;
+                                uint8_t *exps, int8_t *ycodes, uint8_t *yexps, void *ws, esr_stream_t stream) {
+    if (!x || !y || !stat || !ws || !shape_ok(N, HW, C, G) || !(eps >= 0.f) || !codes != !exps || !ycodes != !yexps)
+        return ESR_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
-    GnP p = params(x, nullptr, nullptr, N, HW, C, G, gamma, beta, slope);
-    p.eps = eps;
-    double *partial = (double *)ws, *sums = partial + N * p.splits * 3 * C;
-    colsum<0>(p, partial, sums, st);
-    hipLaunchKernelGGL(gn_groups<0>, dim3(blocks_of(N * G)), dim3(NT), 0, st, p, sums, nullptr, stat);
+    const int V = C % 4 == 0 && aligned({x, y}, {codes, ycodes}) ? 4 : 1;
+    GnP p = params(V, N, HW, C, G, gamma, beta, slope);
+    p.x = x; p.eps = eps;
+    double *partial = (double *)ws;
+    sums<0, false>(p, V, partial, st);
+    finish<0>(p, partial, nullptr, stat, st);
     p.stat = stat;
-    hipLaunchKernelGGL(gn_apply<0>, dim3(blocks_of(N * HW * ((C + 31) / 32 * 32))), dim3(NT), 0, st, p, y, nullptr,
-                       codes, exps);
+    apply<0, false>(p, V, GnOut{y, nullptr, nullptr, nullptr, codes, ycodes, exps, yexps}, st);
     return launched();
 }
 
 extern "C" int esr_gn_lrelu_bwd(const float *x, const int8_t *codes, const uint8_t *exps, const float *gy, int64_t N,
                                 int64_t HW, int32_t C, int32_t G, const float *gamma, const float *beta,
-                                const double *stat, float slope, float *gx, float *g_gamma, float *g_beta, double *sums,
+                                const double *stat, float slope, float *gx, float *g_gamma, float *g_beta, double *sums_,
                                 void *ws, esr_stream_t stream) {
-    if (!bits_ok(x, codes, exps) || !gy || !stat || !sums || !ws || !shape_ok(N, HW, C, G)) return ESR_EINVAL;
+    if (!bits_ok(x, codes, exps) || !gy || !gx || !stat || !sums_ || !ws || !shape_ok(N, HW, C, G)) return ESR_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
-    GnP p = params(x, codes, exps, N, HW, C, G, gamma, beta, slope);
-    p.gy = gy; p.stat = stat;
+    const int V = C % 4 == 0 && aligned({x, gy, gx}, {codes}) ? 4 : 1;
+    GnP p = params(V, N, HW, C, G, gamma, beta, slope);
+    p.x = x; p.codes = codes; p.exps = exps; p.gy = gy; p.stat = stat;
     double *partial = (double *)ws, *grp = partial + N * p.splits * 3 * C + N * 3 * C;
-    colsum<1>(p, partial, sums, st);
-    if (g_gamma || g_beta)
-        hipLaunchKernelGGL(gn_params<1>, dim3(blocks_of(C)), dim3(NT), 0, st, p, sums, nullptr, g_gamma, g_beta);
-    if (gx) {
-        hipLaunchKernelGGL(gn_groups<1>, dim3(blocks_of(N * G)), dim3(NT), 0, st, p, sums, nullptr, grp);
-        p.grp = grp;
-        hipLaunchKernelGGL(gn_apply<1>, dim3(blocks_of(N * HW * ((C + 31) / 32 * 32))), dim3(NT), 0, st, p, gx, nullptr,
-                           nullptr, nullptr);
-    }
+    if (x) sums<1, false>(p, V, partial, st);
+    else sums<1, true>(p, V, partial, st);
+    finish<1>(p, partial, sums_, grp, st);
+    p.grp = grp; p.sums = sums_;
+    const GnOut o{gx, nullptr, g_gamma, g_beta, nullptr, nullptr, nullptr, nullptr};
+    if (x) apply<1, false>(p, V, o, st);
+    else apply<1, true>(p, V, o, st);
     return launched();
 }
 
 extern "C" int esr_gn_lrelu_bwd2(const float *x, const int8_t *codes, const uint8_t *exps, const float *gy,
                                  const float *u, const float *gg_gamma, const float *gg_beta, int64_t N, int64_t HW,
                                  int32_t C, int32_t G, const float *gamma, const float *beta, const double *stat,
-                                 float slope, const double *sums, float *g_x, float *g_gy, float *g_gamma, void *ws,
+                                 float slope, const double *sums_, float *g_x, float *g_gy, float *g_gamma, void *ws,
                                  esr_stream_t stream) {
-    if (!bits_ok(x, codes, exps) || !gy || !stat || !sums || !g_x || !g_gy || !ws || !shape_ok(N, HW, C, G))
+    if (!bits_ok(x, codes, exps) || !gy || !stat || !sums_ || !g_x || !g_gy || !ws || !shape_ok(N, HW, C, G))
         return ESR_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
-    GnP p = params(x, codes, exps, N, HW, C, G, gamma, beta, slope);
-    p.gy = gy; p.u = u; p.gga = gg_gamma; p.ggb = gg_beta; p.stat = stat;
+    const int V = C % 4 == 0 && aligned({x, gy, u, g_x, g_gy}, {codes}) ? 4 : 1;
+    GnP p = params(V, N, HW, C, G, gamma, beta, slope);
+    p.x = x; p.codes = codes; p.exps = exps; p.gy = gy; p.u = u; p.gga = gg_gamma; p.ggb = gg_beta; p.stat = stat;
+    p.sums = sums_;
     double *partial = (double *)ws, *su = partial + N * p.splits * 3 * C, *grp = su + N * 3 * C;
-    if (u) colsum<2>(p, partial, su, st);
-    else su = nullptr;
-    hipLaunchKernelGGL(gn_groups<2>, dim3(blocks_of(N * G)), dim3(NT), 0, st, p, sums, su, grp);
-    p.grp = grp;
-    hipLaunchKernelGGL(gn_apply<2>, dim3(blocks_of(N * HW * ((C + 31) / 32 * 32))), dim3(NT), 0, st, p, g_x, g_gy,
-                       nullptr, nullptr);
-    if (g_gamma) hipLaunchKernelGGL(gn_params<2>, dim3(blocks_of(C)), dim3(NT), 0, st, p, sums, su, g_gamma, nullptr);
+    if (u) {
+        if (x) sums<2, false>(p, V, partial, st);
+        else sums<2, true>(p, V, partial, st);
+    }
+    finish<2>(p, u ? partial : nullptr, su, grp, st);
+    p.grp = grp; p.sums_u = u ? su : nullptr;
+    const GnOut o{g_x, g_gy, g_gamma, nullptr, nullptr, nullptr, nullptr, nullptr};
+    if (x) apply<2, false>(p, V, o, st);
+    else apply<2, true>(p, V, o, st);
     return launched();
 }

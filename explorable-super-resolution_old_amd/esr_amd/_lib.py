@@ -126,7 +126,7 @@ _SIGNATURES = {
                              c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
     'esr_gn_workspace_bytes': [ctypes.c_int64, ctypes.c_int64, c_int, c_int],
     'esr_gn_lrelu_fwd': [c_void_p, ctypes.c_int64, ctypes.c_int64, c_int, c_int, c_void_p, c_void_p, c_float, c_float,
-                         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+                         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     'esr_gn_lrelu_bwd': [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.c_int64, ctypes.c_int64, c_int, c_int,
                          c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                          c_void_p],

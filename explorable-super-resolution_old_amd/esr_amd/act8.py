@@ -5,7 +5,7 @@ them: 8 bytes per activation value in fp32.  `pack` keeps 1 + 1/32: int8 codes t
 channels of a pixel (error <= half a step <= max|x|/127 of the block; x > 0 is kept exactly, so LeakyReLU masks are).
 The backward kernels read the codes themselves: dconv.conv_wgrad_act8 (weight gradients) and gn.group_norm_lrelu
 (checkpoint='int8')."""
-import ctypes
+import contextlib
 
 import torch
 
@@ -22,8 +22,16 @@ def check_mode(mode):
     return mode
 
 
-def _stream(t):
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+_HERE = contextlib.nullcontext()
+
+
+def on(dev):
+    """The context in which launches go to `dev` (entering torch.cuda.device costs several launches' host time)."""
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def stream(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
 
 
 def check_dev(what, *ts):
@@ -74,10 +82,10 @@ class Act8:
             raise RuntimeError('esr_amd.act8: tensors must be on a ROCm device (this build has no CPU path)')
         x = torch.empty(self.shape, device=self.codes.device, dtype=torch.float32)
         if x.numel():
-            with torch.cuda.device(x.device):
+            with on(x.device):
                 _lib.check(_lib.load().esr_act8_unpack(self.codes.data_ptr(), self.exps.data_ptr(),
                                                        x.numel() // self.shape[-1], self.shape[-1], x.data_ptr(),
-                                                       _stream(x)), 'esr_act8_unpack')
+                                                       stream(x.device)), 'esr_act8_unpack')
         return x
 
 
@@ -90,9 +98,9 @@ def pack(x):
     x = x.detach().contiguous()
     codes, exps = empty_blocks(x.shape, x.device)
     if x.numel():
-        with torch.cuda.device(x.device):
+        with on(x.device):
             _lib.check(_lib.load().esr_act8_pack(x.data_ptr(), x.numel() // x.shape[-1], x.shape[-1], codes.data_ptr(),
-                                                 exps.data_ptr(), _stream(x)), 'esr_act8_pack')
+                                                 exps.data_ptr(), stream(x.device)), 'esr_act8_pack')
     return Act8(codes, exps)
 
 

@@ -298,10 +298,10 @@ def conv_wgrad_act8(x8, gy, k, s, p):
         raise RuntimeError('esr_dconv_wgrad_act8_workspace_bytes failed with esr_status %d' % n)
     gw = torch.empty(Co, Ci, k, k, device=gy.device, dtype=torch.float32)
     ws = torch.empty(n, device=gy.device, dtype=torch.uint8)
-    with torch.cuda.device(gy.device):
+    with act8.on(gy.device):
         _lib.check(lib.esr_dconv_wgrad_act8(x8.codes.data_ptr(), x8.exps.data_ptr(), B, H, W, Ci, gy.data_ptr(),
                                             gy.shape[1], gy.shape[2], Co, *geom, gw.data_ptr(), ws.data_ptr(),
-                                            _stream(gy)), 'esr_dconv_wgrad_act8')
+                                            act8.stream(gy.device)), 'esr_dconv_wgrad_act8')
     return gw
 
 

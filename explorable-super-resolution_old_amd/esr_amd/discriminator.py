@@ -125,8 +125,13 @@ def _run(seq, x):
         elif isinstance(m, HipConv2d):
             x = m(x, x8)
         elif isinstance(m, HipGroupNorm) and isinstance(nxt, nn.LeakyReLU):
-            x = m.lrelu(x, nxt.negative_slope)
-            i += 1
+            after = mods[i + 2] if i + 2 < len(mods) else None
+            if isinstance(after, HipConv2d) and after.keeps8():  # its input's 8-bit blocks from the norm's own pass
+                x, x8 = m.lrelu(x, nxt.negative_slope, True)
+            else:
+                x, x8 = m.lrelu(x, nxt.negative_slope), None
+            i += 2
+            continue
         elif FUSED_BN and isinstance(m, nn.BatchNorm2d) and m.training and isinstance(nxt, nn.LeakyReLU) and x.is_cuda:
             x = bn_lrelu(x, m, nxt.negative_slope)
             i += 1

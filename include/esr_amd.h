@@ -482,16 +482,17 @@ int esr_dconv_wgrad_act8(const int8_t *codes, const uint8_t *exps, int64_t B, in
  * x, y, gy, ... [N][HW][C] fp32; G groups of C/G channels; gamma, beta [C] or NULL (1, 0; G = C without them is
  * instance norm).  y = lrelu_slope(γ·(x − μ)·r + β), r = 1/sqrt(v + eps) over each (sample, group).
  * esr_gn_lrelu_fwd writes y and stat [N][G][2] (μ and r, float64) and, where codes / exps are given, x in 8-bit
- *   blocks (above) whose pre-activations keep the sign x's have (a code moves one step where rounding would change it).
- * esr_gn_lrelu_bwd: gx (may be NULL), g_gamma, g_beta (each may be NULL) for upstream gy, and sums [N][2][C] (float64:
+ *   blocks (above) whose pre-activations keep the sign x's have (a code moves one step where rounding would change it);
+ *   where ycodes / yexps are given, y's blocks as esr_act8_pack's.
+ * esr_gn_lrelu_bwd: gx, g_gamma, g_beta (each may be NULL) for upstream gy, and sums [N][2][C] (float64:
  *   Σ gz, Σ gz·x̂ per sample and channel).  The input is x, or codes / exps with x NULL.
  * esr_gn_lrelu_bwd2: the backward of (x, γ, gy) -> (gx, dγ, dβ) (the WGAN-GP double backward, loss.py:244-263) for
  *   upstream u, gg_gamma, gg_beta (each may be NULL = 0) with the sums of esr_gn_lrelu_bwd: g_x, g_gy and g_gamma (may
  *   be NULL).  ws = esr_gn_workspace_bytes(N, HW, C, G) bytes (ESR_EINVAL on bad arguments).  Deterministic. */
 int64_t esr_gn_workspace_bytes(int64_t N, int64_t HW, int32_t C, int32_t G);
 int esr_gn_lrelu_fwd(const float *x, int64_t N, int64_t HW, int32_t C, int32_t G, const float *gamma, const float *beta,
-                     float eps, float slope, float *y, double *stat, int8_t *codes, uint8_t *exps, void *ws,
-                     esr_stream_t stream);
+                     float eps, float slope, float *y, double *stat, int8_t *codes, uint8_t *exps, int8_t *ycodes,
+                     uint8_t *yexps, void *ws, esr_stream_t stream);
 int esr_gn_lrelu_bwd(const float *x, const int8_t *codes, const uint8_t *exps, const float *gy, int64_t N, int64_t HW,
                      int32_t C, int32_t G, const float *gamma, const float *beta, const double *stat, float slope,
                      float *gx, float *g_gamma, float *g_beta, double *sums, void *ws, esr_stream_t stream);

@@ -104,9 +104,11 @@ def test_c_entries_refuse():
     for bad in ((0, 16, 8, 4), (2, 0, 8, 4), (2, 16, 8, 3), (2, 16, 0, 1), (2, 16, 8, 0), (70000, 16, 8, 4),
                 (2, 1 << 40, 64, 4)):
         assert lib.esr_gn_workspace_bytes(*bad) == E
-        assert lib.esr_gn_lrelu_fwd(p, *bad, None, None, 1e-5, 0.2, p, p, None, None, p, None) == E
-    assert lib.esr_gn_lrelu_fwd(p, *ok, None, None, -1.0, 0.2, p, p, None, None, p, None) == E
-    assert lib.esr_gn_lrelu_fwd(p, *ok, None, None, 1e-5, 0.2, p, p, p, None, p, None) == E  # codes without exps
+        assert lib.esr_gn_lrelu_fwd(p, *bad, None, None, 1e-5, 0.2, p, p, None, None, None, None, p, None) == E
+    assert lib.esr_gn_lrelu_fwd(p, *ok, None, None, -1.0, 0.2, p, p, None, None, None, None, p, None) == E
+    for blocks in ((p, None, None, None), (None, None, None, p)):  # codes without exponents
+        assert lib.esr_gn_lrelu_fwd(p, *ok, None, None, 1e-5, 0.2, p, p, *blocks, p, None) == E
+    assert lib.esr_gn_lrelu_bwd(p, None, None, p, *ok, None, None, p, 0.2, None, p, p, p, p, None) == E
     bwd = lambda x, c, e: lib.esr_gn_lrelu_bwd(x, c, e, p, *ok, None, None, p, 0.2, p, p, p, p, p, None)  # noqa: E731
     assert bwd(None, None, None) == E and bwd(p, p, p) == E and bwd(None, p, None) == E
     assert lib.esr_gn_lrelu_bwd2(None, p, p, p, None, None, None, *ok, None, None, p, 0.2, None, p, p, p, p, None) == E

@@ -129,6 +129,21 @@ def test_nonfinite_stays_in_its_group(gpu_device, bad, ck):
     assert bool(gx[hit].isnan().all())
 
 
+@pytest.mark.parametrize('shape,G', SHAPES)
+def test_output_blocks(gpu_device, shape, G):
+    """out8: y's blocks from the norm's pass are act8.pack's of y, y itself unchanged."""
+    c = R.case(shape, G, seed=7, dtype=np.float32)
+    x, w, b = leaves(c, gpu_device)
+    for ck in (None, 'int8'):
+        y, y8 = gn.group_norm_lrelu(x, G, w, b, c.eps, c.slope, ck, out8=True)
+        want = act8.pack(y.permute(0, 2, 3, 1))
+        assert torch.equal(y8.codes, want.codes) and torch.equal(y8.exps, want.exps)
+        plain = gn.group_norm_lrelu(x, G, w, b, c.eps, c.slope, ck)
+        assert torch.equal(y, plain)
+        gy = dev(c.gy, gpu_device)
+        assert torch.equal(torch.autograd.grad(y, x, gy)[0], torch.autograd.grad(plain, x, gy)[0])
+
+
 @pytest.mark.parametrize('ck', [None, 'int8'])
 def test_masks_of_blocks_are_the_forwards(gpu_device, ck):
     """The slope of every value is the forward's, bit for bit: with one group per channel, γ = 1 and M large, gy picks
