@@ -289,9 +289,11 @@ struct GnOut {
 // The elementwise pass.  Workgroups go through samples and rows from the last to the first: what the reduction before
 // read last is still in the 256 MB last-level cache.  The first row block of the first sample also sums the parameter
 // gradients over the samples, in order.
-template <int MODE, int V, bool Q8>
+// BITS: MODE 1, 2: the input is in 8-bit blocks; MODE 0: blocks are written.
+template <int MODE, int V, bool BITS>
 __global__ __launch_bounds__(NT) void gn_apply(GnP p, GnOut o) {
     constexpr int UA = MODE == 2 ? 2 : UN;
+    constexpr bool Q8 = MODE && BITS;
     const int tid = threadIdx.x, lane = tid % p.lanes, ph = tid / p.lanes;
     const int n = p.N - 1 - (int)blockIdx.y, b = p.blocks - 1 - (int)blockIdx.x;
     const int c = ((int)blockIdx.z * NT + lane) * V;
@@ -381,21 +383,19 @@ __global__ __launch_bounds__(NT) void gn_apply(GnP p, GnOut o) {
                 store_f<V>(o.o1, row * p.C + c, a);
                 if constexpr (MODE == 2) store_f<V>(o.o2, row * p.C + c, d);
             }
-            if constexpr (MODE == 0 && !Q8) {
-                if (o.codes || o.ycodes) {
-                    float t[V];
+            if constexpr (MODE == 0 && BITS) {
+                float t[V];
 #pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        t[v] = act ? raw[j].at(v) : 0.f;
-                        a[v] = act ? a[v] : 0.f;
-                    }
-                    if (o.codes)
-                        put_blocks<V>(p, t, act, row, c, lane, o.codes, o.exps, [&](float x, int v) {
-                            return preact(xhat(x, ch.r[v], ch.mu[v]), ch.ga[v], ch.be[v]) > 0.0;
-                        });
-                    if (o.ycodes)
-                        put_blocks<V>(p, a, act, row, c, lane, o.ycodes, o.yexps, [](float y, int) { return y > 0.f; });
+                for (int v = 0; v < V; ++v) {
+                    t[v] = act ? raw[j].at(v) : 0.f;
+                    a[v] = act ? a[v] : 0.f;
                 }
+                if (o.codes)
+                    put_blocks<V>(p, t, act, row, c, lane, o.codes, o.exps, [&](float x, int v) {
+                        return preact(xhat(x, ch.r[v], ch.mu[v]), ch.ga[v], ch.be[v]) > 0.0;
+                    });
+                if (o.ycodes)
+                    put_blocks<V>(p, a, act, row, c, lane, o.ycodes, o.yexps, [](float y, int) { return y > 0.f; });
             }
         }
     }
@@ -428,7 +428,7 @@ GnP params(int V, int64_t N, int64_t HW, int32_t C, int32_t G, const float *gamm
     p.chunks = (lanes + NT - 1) / NT;
     p.lanes = lanes < NT ? lanes : NT;
     p.rpi = NT / p.lanes;
-    // ~4 workgroups per CU for the sums (each leaves K·C float64 partials), 16 for the elementwise pass, of at least UN
+    // ~4 workgroups per CU for the sums (each leaves K·C float64 partials), 8 for the elementwise pass, of at least UN
     // rows per thread
     const int64_t per = (int64_t)N * p.chunks, rows = (HW + UN * p.rpi - 1) / (UN * p.rpi);
     auto cut = [&](int64_t want, int64_t most) {
@@ -437,7 +437,7 @@ GnP params(int V, int64_t N, int64_t HW, int32_t C, int32_t G, const float *gamm
         return (int)(s < most ? s : most);
     };
     p.splits = cut(1024, MAXS);
-    p.blocks = cut(4096, 0x7fffffff);
+    p.blocks = cut(2048, 0x7fffffff);
     return p;
 }
 
@@ -452,11 +452,11 @@ void finish(const GnP &p, const double *partial, double *sums_out, double *out, 
     const int gpb = p.Cg <= 32 ? 32 / p.Cg : 1;
     hipLaunchKernelGGL(gn_finish<MODE>, dim3((p.G + gpb - 1) / gpb, p.N), dim3(NT), 0, st, p, partial, sums_out, out);
 }
-template <int MODE, bool Q8>
+template <int MODE, bool BITS>
 void apply(const GnP &p, int V, const GnOut &o, hipStream_t st) {
     const dim3 grid(p.blocks, p.N, p.chunks);
-    if (V == 4) hipLaunchKernelGGL((gn_apply<MODE, 4, Q8>), grid, dim3(NT), 0, st, p, o);
-    else hipLaunchKernelGGL((gn_apply<MODE, 1, Q8>), grid, dim3(NT), 0, st, p, o);
+    if (V == 4) hipLaunchKernelGGL((gn_apply<MODE, 4, BITS>), grid, dim3(NT), 0, st, p, o);
+    else hipLaunchKernelGGL((gn_apply<MODE, 1, BITS>), grid, dim3(NT), 0, st, p, o);
 }
 
 }  // namespace
@@ -482,7 +482,9 @@ extern "C" int esr_gn_lrelu_fwd(const float *x, int64_t N, int64_t HW, int32_t C
     sums<0, false>(p, V, partial, st);
     finish<0>(p, partial, nullptr, stat, st);
     p.stat = stat;
-    apply<0, false>(p, V, GnOut{y, nullptr, nullptr, nullptr, codes, ycodes, exps, yexps}, st);
+    const GnOut o{y, nullptr, nullptr, nullptr, codes, ycodes, exps, yexps};
+    if (codes || ycodes) apply<0, true>(p, V, o, st);
+    else apply<0, false>(p, V, o, st);
     return launched();
 }
 
