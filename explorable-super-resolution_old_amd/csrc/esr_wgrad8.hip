@@ -1,95 +1,307 @@
 // esr_wgrad8.hip — a convolution's weight gradient from an input kept in 8-bit blocks (esr_act8.h):
 //   gw[co][ci][ky][kx] = Σ_{b, Y, X} x[b, s·Y + ky − p, s·X + kx − p, ci] · dy[b, Y, X, co]   (x zero outside the image)
-// as one matrix product per tap (M = ci, N = co, K = pixels), the codes expanded while they are staged.  Split over the
-// pixels into partials that a second launch adds in a fixed order into torch's weight layout.
+// One matrix product per tap, M = ci, N = co, K = output pixels, on v_mfma_f32_32x32x16_f16.  A code is an integer of 7
+// bits times a power of two, so x is ONE exact f16 number (at a scale of the workgroup's largest exponent; a block more
+// than 2^32 below it counts as zero), and only dy is split, into hi + lo f16 at a power-of-two scale of the largest |dy|
+// so far (|dy − hi − lo| <= 2^-22 |dy| + 2^-39 of that largest): two products where fp32 x takes three, and a quarter of
+// its bytes.  When a tile raises either scale, the float32 accumulators are rescaled by the exact power of two.
+//
+// A workgroup owns 64 ci × 64 co and ALL the taps of a tap group (3×3: nine; 4×4: two rows; 8×8: one row), four waves of
+// one 32×32 tile per tap: dy is expanded once per K step for all of them, and the halo tile of x as well.  K step = RY
+// rows × 16 columns of one image, so that a row of 16 pixels is one MFMA's K and a tap is an LDS address offset.  Both
+// operands lie pixel-major in LDS and are read transposed (ds_read_b64_tr_b16), 32-byte chunks XOR-swizzled by pixel so
+// that the four pixels of a read cover the banks once; at stride 2 the even and the odd columns of x lie apart, which
+// makes a tap's pixels neighbours again.  Two workgroups per CU: one's staging under the other's MFMAs.  The pixels are
+// split over the grid, the partial sums added in a fixed order by a second launch into torch's weight layout.
 #include "esr_act8.h"
 #include "esr_amd.h"
 #include "esr_knobs.h"
 
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-constexpr int NT = 256, KP = 64, PS = 68;
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int NT = 256;
 
 struct WgP {
     const int8_t *codes;
     const uint8_t *exps;
     const float *dy;
-    int B, Hs, Ws, cin, MH, MW, cout, k, s, p, nci, nco;
-    long long per_split;
-    float *partial;  // [splits][taps][nci·64][nco·64]
+    int B, Hs, Ws, cin, nb, MH, MW, cout, k, s, p, nci, nco, groups;
+    int tY, tX, tiles, per_split, splits;  // K steps: rows and columns of tiles per image, all, per split
+    int xvec, gvec;                        // 16-code and float4 loads
+    float *partial;                        // [splits][k·k][nci·64][nco·64]
 };
 
-__global__ __launch_bounds__(NT, 2) void wgrad8_kernel(WgP p) {
-    __shared__ float s_a[KP * PS], s_b[KP * PS];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hl = lane >> 5, ml = lane & 31;
-    const int cob = blockIdx.x % p.nco, cib = blockIdx.x / p.nco % p.nci, t = blockIdx.x / (p.nco * p.nci);
-    const int ky = t / p.k, kx = t % p.k, nb = (p.cin + 31) / 32;
-    const int per_img = p.MH * p.MW;
-    const long long P = (long long)p.B * per_img, k0 = blockIdx.y * p.per_split, k1 = min(P, k0 + p.per_split);
-    const int c = tid & 63, ci = cib * 64 + c, co = cob * 64 + c;
-    const int mt = wave >> 1, nt = wave & 1;
-    f32x16 acc = {};
-    for (long long kb = k0; kb < k1; kb += KP) {
-        __syncthreads();
-        for (int q = wave; q < KP; q += NT / 64) {
-            const long long m = kb + q;
-            float a = 0.f, b = 0.f;
-            if (m < k1) {
-                const int img = (int)(m / per_img), r = (int)(m - (long long)img * per_img);
-                const int Y = r / p.MW, X = r - Y * p.MW, sy = p.s * Y + ky - p.p, sx = p.s * X + kx - p.p;
-                if (ci < p.cin && sy >= 0 && sy < p.Hs && sx >= 0 && sx < p.Ws) {
-                    const long long row = ((long long)img * p.Hs + sy) * p.Ws + sx;
-                    a = act8::value_of((float)p.codes[row * p.cin + ci], p.exps[row * nb + ci / 32]);
-                }
-                if (co < p.cout) b = p.dy[m * p.cout + co];
-            }
-            s_a[q * PS + c] = a;
-            s_b[q * PS + c] = b;
-        }
-        __syncthreads();
-        for (int q = 0; q < KP / 2; ++q)
-            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(s_a[(2 * q + hl) * PS + 32 * mt + ml],
-                                                       s_b[(2 * q + hl) * PS + 32 * nt + ml], acc, 0, 0, 0);
-    }
-    float *dst = p.partial + (((long long)blockIdx.y * p.k * p.k + t) * p.nci * 64 + cib * 64) * p.nco * 64 + cob * 64;
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-        dst[(long long)(32 * mt + (r & 3) + 8 * (r >> 2) + 4 * hl) * p.nco * 64 + 32 * nt + ml] = acc[r];
+__device__ __forceinline__ f16x8 tr_pair(const unsigned char *lds, int at, int step) {
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(lds + at));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(lds + at + step));
+    return __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// gw[co][ci][t] = Σ over splits, in order
-__global__ void wgrad8_reduce(const float *partial, int splits, int T, int cin, int cout, int cip, int cop, float *gw) {
-    const long long i = (long long)blockIdx.x * NT + threadIdx.x, n = (long long)T * cin * cout;
-    if (i >= n) return;
-    const int co = (int)(i % cout), ci = (int)(i / cout % cin), t = (int)(i / ((long long)cout * cin));
+// two codes (bytes b of w ^ 0x80808080) as f16: the byte in the mantissa of 1024, minus 1024 + 128
+__device__ __forceinline__ f16x2 code_pair(uint32_t w, uint32_t sel) {
+    const uint32_t m = __builtin_amdgcn_perm(0x64646464u, w, sel);
+    return __builtin_bit_cast(f16x2, m) - (f16x2){(_Float16)1152.f, (_Float16)1152.f};
+}
+
+// S: the LDS tile's stride between the pixels of a tap; a group of one tap stages exactly its pixels (any stride)
+template <int KR, int KC, int S, int RY>
+struct Shape {
+    static constexpr bool ONE = KR == 1 && KC == 1;
+    static constexpr int ROWS = (RY - 1) * S + KR, COLS = 15 * S + KC;
+    static constexpr int HALF = ((COLS + S - 1) / S + 3) / 4 * 4, PITCH = HALF * S;  // pixels of a row in LDS
+    static constexpr int KPX = RY * 16, XB = ROWS * PITCH * 128, GB = KPX * 256;
+    static constexpr int NX = (ROWS * COLS * 4 + NT - 1) / NT, NG = KPX * 16 / NT;
+};
+
+template <int KR, int KC, int S, int RY>
+__global__ __launch_bounds__(NT, 2) void wgrad8_kernel(WgP p) {
+    using H = Shape<KR, KC, S, RY>;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[H::XB + H::GB];
+    __shared__ unsigned s_red[2][NT / 64][2];
+    unsigned char *s_x = lds, *s_g = lds + H::XB;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hl = lane >> 5;
+    // workgroups of one split share its pixels: they go to one XCD (workgroup ids go round the 8 XCDs)
+    const int work = p.nci * p.nco * p.groups, j8 = blockIdx.x >> 3;
+    const int split = j8 / work * 8 + (blockIdx.x & 7);
+    if (split >= p.splits) return;
+    int w = j8 % work;
+    const int cob = w % p.nco;
+    w /= p.nco;
+    const int cib = w % p.nci, grp = w / p.nci;
+    const int ci0 = cib * 64, co0 = cob * 64;
+    const int tap0 = grp * KR * KC;  // ONE: tap (grp / k, grp % k); else rows grp·KR .. of KC = k taps
+    const int oy = (H::ONE ? grp / p.k : grp * KR) - p.p, ox = (H::ONE ? grp % p.k : 0) - p.p;
+    const int t0 = split * p.per_split, t1 = min(p.tiles, t0 + p.per_split);
+
+    uint4 rx[H::NX];
+    int re[H::NX];
+    f32x4 rg[H::NG];
+    auto load = [&](int t) {
+        const int img = t / (p.tY * p.tX), r = t - img * p.tY * p.tX, ty = r / p.tX;
+        const int Y0 = ty * RY, X0 = (r - ty * p.tX) * 16;
+#pragma unroll
+        for (int j = 0; j < H::NX; ++j) {
+            const int idx = tid + j * NT, px = idx >> 2, ci = ci0 + 16 * (idx & 3), ry = px / H::COLS, cx = px % H::COLS;
+            const int sy = H::ONE ? (Y0 + ry) * p.s + oy : Y0 * S + ry + oy;
+            const int sx = H::ONE ? (X0 + cx) * p.s + ox : X0 * S + cx + ox;
+            rx[j] = make_uint4(0, 0, 0, 0);
+            re[j] = 0;
+            if (ry < H::ROWS && ci < p.cin && sy >= 0 && sy < p.Hs && sx >= 0 && sx < p.Ws) {
+                const long long pix = ((long long)img * p.Hs + sy) * p.Ws + sx;
+                const int8_t *c = p.codes + pix * p.cin + ci;
+                re[j] = p.exps[pix * p.nb + ci / act8::BLK];
+                if (p.xvec) {
+                    rx[j] = *reinterpret_cast<const uint4 *>(c);
+                } else {
+                    uint32_t q[4] = {0, 0, 0, 0};
+                    const int n = min(16, p.cin - ci);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (i < n) q[i >> 2] |= (uint32_t)(uint8_t)c[i] << (8 * (i & 3));
+                    rx[j] = make_uint4(q[0], q[1], q[2], q[3]);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < H::NG; ++j) {
+            const int idx = tid + j * NT, q = idx >> 4, co = co0 + 4 * (idx & 15), Y = Y0 + (q >> 4), X = X0 + (q & 15);
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            if (Y < p.MH && X < p.MW && co < p.cout) {
+                const float *g = p.dy + (((long long)img * p.MH + Y) * p.MW + X) * p.cout + co;
+                if (p.gvec) {
+                    v = *reinterpret_cast<const f32x4 *>(g);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (co + i < p.cout) v[i] = g[i];
+                }
+            }
+            rg[j] = v;
+        }
+    };
+    // the tile's largest exponent byte and |dy| (finite ones), published for all waves
+    auto publish = [&](int slot) {
+        unsigned me = 0, mg = 0;
+#pragma unroll
+        for (int j = 0; j < H::NX; ++j) me = max(me, re[j] == 255 ? 0u : (unsigned)re[j]);
+#pragma unroll
+        for (int j = 0; j < H::NG; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mg = max(mg, act8::abs_bits(rg[j][i]));
+        if (__any(mg >= 0x7f800000u)) {
+            mg = 0;
+#pragma unroll
+            for (int j = 0; j < H::NG; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const unsigned b = act8::abs_bits(rg[j][i]);
+                    mg = max(mg, b >= 0x7f800000u ? 0u : b);
+                }
+        }
+        me = act8::block_max<64>(me);
+        mg = act8::block_max<64>(mg);
+        if (lane == 0) {
+            s_red[slot][wave][0] = me;
+            s_red[slot][wave][1] = mg;
+        }
+    };
+
+    f32x16 acc[KR * KC];
+#pragma unroll
+    for (int t = 0; t < KR * KC; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
+    int ex = 0, eg = -110;  // x is staged at 2^(132 + 8 − ex), dy at 2^(15 − eg), |dy| < 2^eg
+
+    // transposed-read lane roles: pixel rq of four, channels 16·(group of 16 lanes) + 4·(lane & 3) of a 32-channel tile
+    const int wm = wave >> 1, wn = wave & 1, i16 = lane & 15, rq = i16 >> 2;
+    const int cb = 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+    int ax[KC];
+#pragma unroll
+    for (int b = 0; b < KC; ++b) {
+        const int pos = (b % S) * H::HALF + 8 * hl + rq + b / S, c = 32 * wm + cb;
+        ax[b] = pos * 128 + (((c >> 4) ^ (2 * ((pos >> 1) & 1))) << 5) + (c & 15) * 2;
+    }
+    const int cg = 32 * wn + cb, ag = (8 * hl + rq) * 256 + (((cg >> 4) ^ (2 * rq)) << 5) + (cg & 15) * 2;
+
+    if (t0 < t1) load(t0);
+    for (int t = t0; t < t1; ++t) {
+        const int slot = (t - t0) & 1;
+        publish(slot);
+        __syncthreads();  // everyone is done with the tile before, and the maxima are there
+        unsigned me = 0, mg = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) {
+            me = max(me, s_red[slot][i][0]);
+            mg = max(mg, s_red[slot][i][1]);
+        }
+        const int ex2 = max(ex, (int)me), eg2 = max(eg, (int)(mg >> 23) - 126), down = ex2 - ex + eg2 - eg;
+        if (down) {
+#pragma unroll
+            for (int q = 0; q < KR * KC; ++q)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[q][r] = ldexpf(acc[q][r], -down);
+        }
+        ex = ex2;
+        eg = eg2;
+        const float sg = ldexpf(1.f, 15 - eg);
+#pragma unroll
+        for (int j = 0; j < H::NX; ++j) {
+            const int idx = tid + j * NT, px = idx >> 2, ry = px / H::COLS, cx = px % H::COLS;
+            if (ry >= H::ROWS) break;
+            const int pos = (cx % S) * H::HALF + cx / S;
+            const _Float16 sc = re[j] == 255 ? (_Float16)__builtin_nanf("") : (_Float16)ldexpf(1.f, max(re[j] - ex, -40) + 8);
+            const f16x2 s2 = {sc, sc};
+            const uint32_t q[4] = {rx[j].x, rx[j].y, rx[j].z, rx[j].w};
+            f16x2 o[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t u = q[i] ^ 0x80808080u;
+                o[2 * i] = code_pair(u, 0x04010400u) * s2;
+                o[2 * i + 1] = code_pair(u, 0x04030402u) * s2;
+            }
+            unsigned char *d = s_x + (ry * H::PITCH + pos) * 128 + (((idx & 3) ^ (2 * ((pos >> 1) & 1))) << 5);
+            *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<const uint4 *>(&o[0]);
+            *reinterpret_cast<uint4 *>(d + 16) = *reinterpret_cast<const uint4 *>(&o[4]);
+        }
+#pragma unroll
+        for (int j = 0; j < H::NG; ++j) {
+            const int idx = tid + j * NT, q = idx >> 4, c = 4 * (idx & 15);
+            f16x4 h, l;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float v = rg[j][i] * sg;
+                h[i] = (_Float16)v;
+                l[i] = (_Float16)(v - (float)h[i]);
+            }
+            const int d = q * 256 + (((c >> 4) ^ (2 * (q & 3))) << 5) + (c & 15) * 2;
+            *reinterpret_cast<f16x4 *>(s_g + d) = h;
+            *reinterpret_cast<f16x4 *>(s_g + (d ^ 128)) = l;
+        }
+        __syncthreads();
+        if (t + 1 < t1) load(t + 1);
+#pragma unroll
+        for (int kq = 0; kq < RY; ++kq) {
+            const f16x8 gh = tr_pair(s_g, ag + kq * 4096, 1024), gl = tr_pair(s_g, (ag ^ 128) + kq * 4096, 1024);
+#pragma unroll
+            for (int a = 0; a < KR; ++a)
+#pragma unroll
+                for (int b = 0; b < KC; ++b) {
+                    const f16x8 x = tr_pair(s_x, ax[b] + (kq * S + a) * H::PITCH * 128, 512);
+                    acc[a * KC + b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, gl, acc[a * KC + b], 0, 0, 0);
+                    acc[a * KC + b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, gh, acc[a * KC + b], 0, 0, 0);
+                }
+        }
+    }
+    const int cip = p.nci * 64, cop = p.nco * 64, back = ex - 140 + eg - 15;
+    float *dst = p.partial + (((long long)split * p.k * p.k + tap0) * cip + ci0 + 32 * wm) * cop + co0 + 32 * wn + (lane & 31);
+#pragma unroll
+    for (int t = 0; t < KR * KC; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            dst[((long long)t * cip + (r & 3) + 8 * (r >> 2) + 4 * hl) * cop] = ldexpf(acc[t][r], back);
+}
+
+// gw[co][ci][t] = Σ over the splits: 32 consecutive co × 8 slices of the splits, a slice in order, then the slices
+__global__ __launch_bounds__(NT) void wgrad8_reduce(const float *partial, int splits, int T, int cin, int cout, int cip,
+                                                    int cop, float *gw) {
+    __shared__ float sl[8][32];
+    const int q = threadIdx.x >> 5, o = threadIdx.x & 31, nco = (cout + 31) / 32;
+    const int co = blockIdx.x % nco * 32 + o, row = blockIdx.x / nco, ci = row % cin, t = row / cin;
+    const long long step = (long long)T * cip * cop;
+    const float *src = partial + ((long long)t * cip + ci) * cop + co;
+    const int s0 = splits * q / 8, s1 = splits * (q + 1) / 8;
     float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += partial[(((long long)s * T + t) * cip + ci) * cop + co];
-    gw[((long long)co * cin + ci) * T + t] = v;
+    if (co < cout)
+#pragma unroll 8
+        for (int s = s0; s < s1; ++s) v += src[s * step];
+    sl[q][o] = v;
+    __syncthreads();
+    if (q == 0 && co < cout) {
+        for (int r = 1; r < 8; ++r) v += sl[r][o];
+        gw[((long long)co * cin + ci) * T + t] = v;
+    }
 }
 
 struct Geo {
-    int nci, nco, T, splits;
-    long long P, per_split;
+    int kind, ry;  // 0: 3×3, 1: 4×4 stride 2, 2: 4×4 stride 1, 3: 8×8, 4: tap by tap
+    WgP p;
 };
 bool geometry(int64_t B, int32_t Hs, int32_t Ws, int32_t cin, int32_t MH, int32_t MW, int32_t cout, int32_t k,
               int32_t s, int32_t pad, Geo &g) {
     if (B <= 0 || Hs <= 0 || Ws <= 0 || cin <= 0 || MH <= 0 || MW <= 0 || cout <= 0 || k <= 0 || s <= 0 || pad < 0)
         return false;
-    if (k > 8 || Hs > 65535 || Ws > 65535 || pad > 65535 || s > 65535 || cin > 65536 || cout > 65536) return false;
-    if (MH != (Hs + 2 * pad - k) / s + 1 || MW != (Ws + 2 * pad - k) / s + 1 || Hs + 2 * pad < k || Ws + 2 * pad < k)
-        return false;
+    if (k > 8 || Hs > 65535 || Ws > 65535 || pad > 8192 || s > 8192 || cin > 65536 || cout > 65536) return false;
+    if (Hs + 2 * pad < k || Ws + 2 * pad < k) return false;
+    if (MH != (Hs + 2 * pad - k) / s + 1 || MW != (Ws + 2 * pad - k) / s + 1) return false;
     if (B > 0x7fffffffLL / ((int64_t)MH * MW) || B > 0x7fffffffLL / ((int64_t)Hs * Ws)) return false;
-    g.nci = (cin + 63) / 64;
-    g.nco = (cout + 63) / 64;
-    g.T = k * k;
-    g.P = B * MH * MW;
-    const long long tiles = (long long)g.nci * g.nco * g.T;
-    long long n = (1024 + tiles - 1) / tiles, most = (g.P + 4 * KP - 1) / (4 * KP);
-    n = n < most ? n : most;
-    g.per_split = ((g.P + n - 1) / n + KP - 1) / KP * KP;
-    g.splits = (int)((g.P + g.per_split - 1) / g.per_split);
-    return tiles <= 0x7fffffffLL;
+    g.kind = k == 3 && s == 1 ? 0 : k == 4 && s == 2 ? 1 : k == 4 && s == 1 ? 2 : k == 8 && s == 1 ? 3 : 4;
+    g.ry = g.kind == 1 ? 4 : 8;
+    WgP &p = g.p;
+    p = WgP{};
+    p.B = (int)B; p.Hs = Hs; p.Ws = Ws; p.cin = cin; p.nb = (cin + 31) / 32; p.MH = MH; p.MW = MW; p.cout = cout;
+    p.k = k; p.s = s; p.p = pad;
+    p.nci = (cin + 63) / 64;
+    p.nco = (cout + 63) / 64;
+    p.groups = g.kind == 0 ? 1 : g.kind <= 2 ? 2 : g.kind == 3 ? 8 : k * k;
+    p.tY = (MH + g.ry - 1) / g.ry;
+    p.tX = (MW + 15) / 16;
+    const long long tiles = B * p.tY * p.tX, work = (long long)p.nci * p.nco * p.groups;
+    if (tiles > 0x7fffffffLL || work > (1 << 24)) return false;
+    p.tiles = (int)tiles;
+    // two workgroups per CU, a K step each at least
+    const long long n = work >= 512 ? 1 : 512 / work;
+    p.per_split = (int)((tiles + (n < tiles ? n : tiles) - 1) / (n < tiles ? n : tiles));
+    p.splits = (p.tiles + p.per_split - 1) / p.per_split;
+    return (long long)(p.splits + 7) / 8 * 8 * work <= 0x7fffffffLL;
 }
 
 }  // namespace
@@ -98,7 +310,7 @@ extern "C" int64_t esr_dconv_wgrad_act8_workspace_bytes(int64_t B, int32_t Hs, i
                                                         int32_t MW, int32_t cout, int32_t k, int32_t s, int32_t pad) {
     Geo g;
     if (!geometry(B, Hs, Ws, cin, MH, MW, cout, k, s, pad, g)) return ESR_EINVAL;
-    return 4LL * g.splits * g.T * g.nci * 64 * g.nco * 64;
+    return 4LL * g.p.splits * k * k * g.p.nci * 64 * g.p.nco * 64;
 }
 
 extern "C" int esr_dconv_wgrad_act8(const int8_t *codes, const uint8_t *exps, int64_t B, int32_t Hs, int32_t Ws,
@@ -107,10 +319,19 @@ extern "C" int esr_dconv_wgrad_act8(const int8_t *codes, const uint8_t *exps, in
     Geo g;
     if (!codes || !exps || !dy || !gw || !ws || !geometry(B, Hs, Ws, cin, MH, MW, cout, k, s, pad, g)) return ESR_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
-    WgP p{codes, exps, dy, (int)B, Hs, Ws, cin, MH, MW, cout, k, s, pad, g.nci, g.nco, g.per_split, (float *)ws};
-    hipLaunchKernelGGL(wgrad8_kernel, dim3(g.nci * g.nco * g.T, g.splits), dim3(NT), 0, st, p);
-    const long long n = (long long)g.T * cin * cout;
-    hipLaunchKernelGGL(wgrad8_reduce, dim3((unsigned)((n + NT - 1) / NT)), dim3(NT), 0, st, p.partial, g.splits, g.T,
-                       cin, cout, g.nci * 64, g.nco * 64, gw);
+    WgP &p = g.p;
+    p.codes = codes; p.exps = exps; p.dy = dy; p.partial = (float *)ws;
+    p.xvec = cin % 16 == 0 && (uintptr_t)codes % 16 == 0;
+    p.gvec = cout % 4 == 0 && (uintptr_t)dy % 16 == 0;
+    const dim3 grid((unsigned)((p.splits + 7) / 8 * 8 * p.nci * p.nco * p.groups)), block(NT);
+    switch (g.kind) {
+        case 0: hipLaunchKernelGGL((wgrad8_kernel<3, 3, 1, 8>), grid, block, 0, st, p); break;
+        case 1: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 2, 4>), grid, block, 0, st, p); break;
+        case 2: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 1, 8>), grid, block, 0, st, p); break;
+        case 3: hipLaunchKernelGGL((wgrad8_kernel<1, 8, 1, 8>), grid, block, 0, st, p); break;
+        default: hipLaunchKernelGGL((wgrad8_kernel<1, 1, 1, 8>), grid, block, 0, st, p);
+    }
+    hipLaunchKernelGGL(wgrad8_reduce, dim3((unsigned)((cout + 31) / 32) * cin * k * k), block, 0, st, p.partial, p.splits,
+                       k * k, cin, cout, p.nci * 64, p.nco * 64, gw);
     return hipGetLastError() == hipSuccess ? ESR_OK : ESR_ELAUNCH;
 }
