@@ -3,16 +3,20 @@
 // One matrix product per tap, M = ci, N = co, K = output pixels, on v_mfma_f32_32x32x16_f16.  A code is an integer of 7
 // bits times a power of two, so x is ONE exact f16 number (at a scale of the workgroup's largest exponent; a block more
 // than 2^32 below it counts as zero), and only dy is split, into hi + lo f16 at a power-of-two scale of the largest |dy|
-// so far (|dy − hi − lo| <= 2^-22 |dy| + 2^-39 of that largest): two products where fp32 x takes three, and a quarter of
-// its bytes.  When a tile raises either scale, the float32 accumulators are rescaled by the exact power of two.
+// so far (|dy − hi − lo| <= 2^-22 |dy| + 2^-36 of that largest): two products where fp32 x takes three, and a quarter of
+// its bytes.  The scales leave room for a growth of 2^4 (dy) and 2^2 (x); a tile beyond that raises a flag, and the
+// workgroup finds its maxima, rescales the float32 accumulators by the exact power of two and stages the tile again.
 //
-// A workgroup owns 64 ci × 64 co and ALL the taps of a tap group (3×3: nine; 4×4: two rows; 8×8: one row), four waves of
-// one 32×32 tile per tap: dy is expanded once per K step for all of them, and the halo tile of x as well.  K step = RY
-// rows × 16 columns of one image, so that a row of 16 pixels is one MFMA's K and a tap is an LDS address offset.  Both
-// operands lie pixel-major in LDS and are read transposed (ds_read_b64_tr_b16), 32-byte chunks XOR-swizzled by pixel so
-// that the four pixels of a read cover the banks once; at stride 2 the even and the odd columns of x lie apart, which
-// makes a tap's pixels neighbours again.  Two workgroups per CU: one's staging under the other's MFMAs.  The pixels are
-// split over the grid, the partial sums added in a fixed order by a second launch into torch's weight layout.
+// A workgroup owns 64 ci × 64 co and ALL the taps of a tap group (3×3: nine; 4×4 stride 2: sixteen; 4×4 stride 1: two
+// rows; 8×8: one row), a wave one 32×32 tile for each of up to nine taps: dy is expanded once per K step for all of
+// them, and the halo tile of x as well.  K step = RY rows × 16 columns of one image, so that a row of 16 pixels is one
+// MFMA's K and a tap is an LDS address offset.  Both operands lie pixel-major in LDS and are read transposed
+// (ds_read_b64_tr_b16), 32-byte chunks XOR-swizzled by pixel so that the four pixels of a read cover the banks once; at
+// stride 2 the even and the odd columns of x lie apart, which makes a tap's pixels neighbours again.  Two LDS tiles: one
+// is multiplied while the next is expanded into the other and the one after that is on its way into registers, one
+// barrier per step.  Two workgroups of four waves share a CU (4×4 stride 2: one of eight, half of whose waves multiply
+// first and expand second), so that one's expansion runs under the other's MFMAs.  The pixels are split over the grid,
+// the partial sums added in a fixed order by a second launch into torch's weight layout.
 #include "esr_act8.h"
 #include "esr_amd.h"
 #include "esr_knobs.h"
@@ -45,28 +49,31 @@ __device__ __forceinline__ f16x8 tr_pair(const unsigned char *lds, int at, int s
     return __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// two codes (bytes b of w ^ 0x80808080) as f16: the byte in the mantissa of 1024, minus 1024 + 128
-__device__ __forceinline__ f16x2 code_pair(uint32_t w, uint32_t sel) {
-    const uint32_t m = __builtin_amdgcn_perm(0x64646464u, w, sel);
-    return __builtin_bit_cast(f16x2, m) - (f16x2){(_Float16)1152.f, (_Float16)1152.f};
+// two codes (bytes of w ^ 0x80808080, picked by sel) times s as f16: the byte in the mantissa of 1024 is 1024 + 128 +
+// code, and one fused multiply-add leaves the exact code·s (s a power of two <= 2^5; off = −1152·s)
+__device__ __forceinline__ f16x2 code_pair(uint32_t w, uint32_t sel, f16x2 s, f16x2 off) {
+    return __builtin_elementwise_fma(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, sel)), s, off);
 }
 
-// S: the LDS tile's stride between the pixels of a tap; a group of one tap stages exactly its pixels (any stride)
-template <int KR, int KC, int S, int RY>
+// S: the LDS tile's stride between the pixels of a tap; a group of one tap stages exactly its pixels (any stride).
+// TG: tap groups of a workgroup, four waves each.
+template <int KR, int KC, int S, int TG>
 struct Shape {
     static constexpr bool ONE = KR == 1 && KC == 1;
-    static constexpr int ROWS = (RY - 1) * S + KR, COLS = 15 * S + KC;
+    static constexpr int RY = 4, NT = 256 * TG;
+    static constexpr int ROWS = (RY - 1) * S + KR * TG, COLS = 15 * S + KC;
     static constexpr int HALF = ((COLS + S - 1) / S + 3) / 4 * 4, PITCH = HALF * S;  // pixels of a row in LDS
-    static constexpr int KPX = RY * 16, XB = ROWS * PITCH * 128, GB = KPX * 256;
+    static constexpr int KPX = RY * 16, XB = ROWS * PITCH * 128, BUF = XB + KPX * 256;
     static constexpr int NX = (ROWS * COLS * 4 + NT - 1) / NT, NG = KPX * 16 / NT;
 };
 
-template <int KR, int KC, int S, int RY>
-__global__ __launch_bounds__(NT, 2) void wgrad8_kernel(WgP p) {
-    using H = Shape<KR, KC, S, RY>;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[H::XB + H::GB];
-    __shared__ unsigned s_red[2][NT / 64][2];
-    unsigned char *s_x = lds, *s_g = lds + H::XB;
+template <int KR, int KC, int S, int TG>
+__global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
+    using H = Shape<KR, KC, S, TG>;
+    constexpr int RY = H::RY;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * H::BUF];
+    __shared__ unsigned s_red[4 * TG][2];
+    __shared__ int s_flag[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hl = lane >> 5;
     // workgroups of one split share its pixels: they go to one XCD (workgroup ids go round the 8 XCDs)
     const int work = p.nci * p.nco * p.groups, j8 = blockIdx.x >> 3;
@@ -77,25 +84,33 @@ __global__ __launch_bounds__(NT, 2) void wgrad8_kernel(WgP p) {
     w /= p.nco;
     const int cib = w % p.nci, grp = w / p.nci;
     const int ci0 = cib * 64, co0 = cob * 64;
-    const int tap0 = grp * KR * KC;  // ONE: tap (grp / k, grp % k); else rows grp·KR .. of KC = k taps
-    const int oy = (H::ONE ? grp / p.k : grp * KR) - p.p, ox = (H::ONE ? grp % p.k : 0) - p.p;
+    const int oy = (H::ONE ? grp / p.k : grp * KR * TG) - p.p, ox = (H::ONE ? grp % p.k : 0) - p.p;
     const int t0 = split * p.per_split, t1 = min(p.tiles, t0 + p.per_split);
 
+    // this thread's places: x pixel (row, column) and its 16 channels, their bytes in the LDS tile
+    int xr[H::NX], xd[H::NX];
+#pragma unroll
+    for (int j = 0; j < H::NX; ++j) {
+        const int idx = tid + j * H::NT, px = idx >> 2, ry = px / H::COLS, cx = px % H::COLS;
+        const int pos = cx % S * H::HALF + cx / S;
+        xr[j] = ry < H::ROWS && ci0 + 16 * (idx & 3) < p.cin ? ry << 16 | cx : -1;
+        xd[j] = ry < H::ROWS ? (ry * H::PITCH + pos) * 128 + (((idx & 3) ^ (2 * ((pos >> 1) & 1))) << 5) : -1;
+    }
     uint4 rx[H::NX];
     int re[H::NX];
     f32x4 rg[H::NG];
     auto load = [&](int t) {
         const int img = t / (p.tY * p.tX), r = t - img * p.tY * p.tX, ty = r / p.tX;
         const int Y0 = ty * RY, X0 = (r - ty * p.tX) * 16;
+        const int st = H::ONE ? p.s : 1, ys = Y0 * (H::ONE ? p.s : S) + oy, xs = X0 * (H::ONE ? p.s : S) + ox;
 #pragma unroll
         for (int j = 0; j < H::NX; ++j) {
-            const int idx = tid + j * NT, px = idx >> 2, ci = ci0 + 16 * (idx & 3), ry = px / H::COLS, cx = px % H::COLS;
-            const int sy = H::ONE ? (Y0 + ry) * p.s + oy : Y0 * S + ry + oy;
-            const int sx = H::ONE ? (X0 + cx) * p.s + ox : X0 * S + cx + ox;
+            const int sy = ys + (xr[j] >> 16) * st, sx = xs + (xr[j] & 0xffff) * st;
             rx[j] = make_uint4(0, 0, 0, 0);
             re[j] = 0;
-            if (ry < H::ROWS && ci < p.cin && sy >= 0 && sy < p.Hs && sx >= 0 && sx < p.Ws) {
-                const long long pix = ((long long)img * p.Hs + sy) * p.Ws + sx;
+            if (xr[j] >= 0 && (unsigned)sy < (unsigned)p.Hs && (unsigned)sx < (unsigned)p.Ws) {
+                const int ci = ci0 + 16 * (tid & 3);
+                const long long pix = (img * p.Hs + sy) * p.Ws + sx;
                 const int8_t *c = p.codes + pix * p.cin + ci;
                 re[j] = p.exps[pix * p.nb + ci / act8::BLK];
                 if (p.xvec) {
@@ -112,10 +127,10 @@ __global__ __launch_bounds__(NT, 2) void wgrad8_kernel(WgP p) {
         }
 #pragma unroll
         for (int j = 0; j < H::NG; ++j) {
-            const int idx = tid + j * NT, q = idx >> 4, co = co0 + 4 * (idx & 15), Y = Y0 + (q >> 4), X = X0 + (q & 15);
+            const int idx = tid + j * H::NT, q = idx >> 4, co = co0 + 4 * (idx & 15), Y = Y0 + (q >> 4), X = X0 + (q & 15);
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
             if (Y < p.MH && X < p.MW && co < p.cout) {
-                const float *g = p.dy + (((long long)img * p.MH + Y) * p.MW + X) * p.cout + co;
+                const float *g = p.dy + (long long)((img * p.MH + Y) * p.MW + X) * p.cout + co;
                 if (p.gvec) {
                     v = *reinterpret_cast<const f32x4 *>(g);
                 } else {
@@ -127,121 +142,144 @@ __global__ __launch_bounds__(NT, 2) void wgrad8_kernel(WgP p) {
             rg[j] = v;
         }
     };
-    // the tile's largest exponent byte and |dy| (finite ones), published for all waves
-    auto publish = [&](int slot) {
-        unsigned me = 0, mg = 0;
-#pragma unroll
-        for (int j = 0; j < H::NX; ++j) me = max(me, re[j] == 255 ? 0u : (unsigned)re[j]);
-#pragma unroll
-        for (int j = 0; j < H::NG; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mg = max(mg, act8::abs_bits(rg[j][i]));
-        if (__any(mg >= 0x7f800000u)) {
-            mg = 0;
-#pragma unroll
-            for (int j = 0; j < H::NG; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const unsigned b = act8::abs_bits(rg[j][i]);
-                    mg = max(mg, b >= 0x7f800000u ? 0u : b);
-                }
-        }
-        me = act8::block_max<64>(me);
-        mg = act8::block_max<64>(mg);
-        if (lane == 0) {
-            s_red[slot][wave][0] = me;
-            s_red[slot][wave][1] = mg;
-        }
-    };
 
     f32x16 acc[KR * KC];
 #pragma unroll
     for (int t = 0; t < KR * KC; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
-    int ex = 0, eg = -110;  // x is staged at 2^(132 + 8 − ex), dy at 2^(15 − eg), |dy| < 2^eg
+    int ex = 0, eg = -110;  // x is staged at 2^(135 − ex), dy at 2^(11 − eg)
 
-    // transposed-read lane roles: pixel rq of four, channels 16·(group of 16 lanes) + 4·(lane & 3) of a 32-channel tile
-    const int wm = wave >> 1, wn = wave & 1, i16 = lane & 15, rq = i16 >> 2;
-    const int cb = 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
-    int ax[KC];
-#pragma unroll
-    for (int b = 0; b < KC; ++b) {
-        const int pos = (b % S) * H::HALF + 8 * hl + rq + b / S, c = 32 * wm + cb;
-        ax[b] = pos * 128 + (((c >> 4) ^ (2 * ((pos >> 1) & 1))) << 5) + (c & 15) * 2;
-    }
-    const int cg = 32 * wn + cb, ag = (8 * hl + rq) * 256 + (((cg >> 4) ^ (2 * rq)) << 5) + (cg & 15) * 2;
-
-    if (t0 < t1) load(t0);
-    for (int t = t0; t < t1; ++t) {
-        const int slot = (t - t0) & 1;
-        publish(slot);
-        __syncthreads();  // everyone is done with the tile before, and the maxima are there
+    // The loaded tile's largest exponent byte and |dy| (finite ones) over the workgroup; the scales raised to them.
+    auto rescale = [&]() {
         unsigned me = 0, mg = 0;
 #pragma unroll
-        for (int i = 0; i < NT / 64; ++i) {
-            me = max(me, s_red[slot][i][0]);
-            mg = max(mg, s_red[slot][i][1]);
+        for (int j = 0; j < H::NX; ++j) me = max(me, re[j] == 255 ? 0u : (unsigned)re[j]);
+#pragma unroll
+        for (int j = 0; j < H::NG; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned b = act8::abs_bits(rg[j][i]);
+                mg = max(mg, b >= 0x7f800000u ? 0u : b);
+            }
+        me = act8::block_max<64>(me);
+        mg = act8::block_max<64>(mg);
+        if (lane == 0) {
+            s_red[wave][0] = me;
+            s_red[wave][1] = mg;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4 * TG; ++i) {
+            me = max(me, s_red[i][0]);
+            mg = max(mg, s_red[i][1]);
         }
         const int ex2 = max(ex, (int)me), eg2 = max(eg, (int)(mg >> 23) - 126), down = ex2 - ex + eg2 - eg;
-        if (down) {
 #pragma unroll
-            for (int q = 0; q < KR * KC; ++q)
+        for (int q = 0; q < KR * KC; ++q)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[q][r] = ldexpf(acc[q][r], -down);
-        }
+            for (int r = 0; r < 16; ++r) acc[q][r] = ldexpf(acc[q][r], -down);
         ex = ex2;
         eg = eg2;
-        const float sg = ldexpf(1.f, 15 - eg);
+    };
+    // The loaded tile into an LDS tile; whether one of this thread's values is beyond the scales.
+    auto expand = [&](unsigned char *buf) {
+        int me = 0;
 #pragma unroll
         for (int j = 0; j < H::NX; ++j) {
-            const int idx = tid + j * NT, px = idx >> 2, ry = px / H::COLS, cx = px % H::COLS;
-            if (ry >= H::ROWS) break;
-            const int pos = (cx % S) * H::HALF + cx / S;
-            const _Float16 sc = re[j] == 255 ? (_Float16)__builtin_nanf("") : (_Float16)ldexpf(1.f, max(re[j] - ex, -40) + 8);
-            const f16x2 s2 = {sc, sc};
+            if (xd[j] < 0) break;
+            me = max(me, re[j] == 255 ? 0 : re[j]);
+            const _Float16 sc = re[j] == 255 ? (_Float16)__builtin_nanf("") : (_Float16)ldexpf(1.f, min(re[j] - ex, 2) + 3);
+            const f16x2 s = {sc, sc}, off = s * (_Float16)-1152.f;
             const uint32_t q[4] = {rx[j].x, rx[j].y, rx[j].z, rx[j].w};
             f16x2 o[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t u = q[i] ^ 0x80808080u;
-                o[2 * i] = code_pair(u, 0x04010400u) * s2;
-                o[2 * i + 1] = code_pair(u, 0x04030402u) * s2;
+                o[2 * i] = code_pair(u, 0x04010400u, s, off);
+                o[2 * i + 1] = code_pair(u, 0x04030402u, s, off);
             }
-            unsigned char *d = s_x + (ry * H::PITCH + pos) * 128 + (((idx & 3) ^ (2 * ((pos >> 1) & 1))) << 5);
-            *reinterpret_cast<uint4 *>(d) = *reinterpret_cast<const uint4 *>(&o[0]);
-            *reinterpret_cast<uint4 *>(d + 16) = *reinterpret_cast<const uint4 *>(&o[4]);
+            *reinterpret_cast<uint4 *>(buf + xd[j]) = *reinterpret_cast<const uint4 *>(&o[0]);
+            *reinterpret_cast<uint4 *>(buf + xd[j] + 16) = *reinterpret_cast<const uint4 *>(&o[4]);
         }
+        unsigned mg = 0;
+        const float sg = ldexpf(1.f, 11 - eg);
 #pragma unroll
         for (int j = 0; j < H::NG; ++j) {
-            const int idx = tid + j * NT, q = idx >> 4, c = 4 * (idx & 15);
+            const int idx = tid + j * H::NT, q = idx >> 4, c = 4 * (idx & 15);
             f16x4 h, l;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+                mg = max(mg, act8::abs_bits(rg[j][i]));
                 const float v = rg[j][i] * sg;
                 h[i] = (_Float16)v;
                 l[i] = (_Float16)(v - (float)h[i]);
             }
-            const int d = q * 256 + (((c >> 4) ^ (2 * (q & 3))) << 5) + (c & 15) * 2;
-            *reinterpret_cast<f16x4 *>(s_g + d) = h;
-            *reinterpret_cast<f16x4 *>(s_g + (d ^ 128)) = l;
+            const int d = H::XB + q * 256 + (((c >> 4) ^ (2 * (q & 3))) << 5) + (c & 15) * 2;
+            *reinterpret_cast<f16x4 *>(buf + d) = h;
+            *reinterpret_cast<f16x4 *>(buf + (((d - H::XB) ^ 128) + H::XB)) = l;
         }
-        __syncthreads();
-        if (t + 1 < t1) load(t + 1);
+        return me > ex + 2 || (int)(mg >> 23) - 126 > eg + 4;
+    };
+
+    // transposed-read lane roles: pixel rq of four, channels 16·(group of 16 lanes) + 4·(lane & 3) of a 32-channel tile
+    const int wm = (wave >> 1) & 1, wn = wave & 1, tg = TG > 1 ? wave >> 2 : 0, i16 = lane & 15, rq = i16 >> 2;
+    const int cb = 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+    int ax[KC];
+#pragma unroll
+    for (int b = 0; b < KC; ++b) {
+        const int pos = (b % S) * H::HALF + 8 * hl + rq + b / S, c = 32 * wm + cb;
+        ax[b] = (tg * KR * H::PITCH + pos) * 128 + (((c >> 4) ^ (2 * ((pos >> 1) & 1))) << 5) + (c & 15) * 2;
+    }
+    const int cg = 32 * wn + cb, ag = (8 * hl + rq) * 256 + (((cg >> 4) ^ (2 * rq)) << 5) + (cg & 15) * 2;
+    auto multiply = [&](const unsigned char *buf) {
 #pragma unroll
         for (int kq = 0; kq < RY; ++kq) {
-            const f16x8 gh = tr_pair(s_g, ag + kq * 4096, 1024), gl = tr_pair(s_g, (ag ^ 128) + kq * 4096, 1024);
+            const f16x8 gh = tr_pair(buf + H::XB, ag + kq * 4096, 1024), gl = tr_pair(buf + H::XB, (ag ^ 128) + kq * 4096, 1024);
 #pragma unroll
             for (int a = 0; a < KR; ++a)
 #pragma unroll
                 for (int b = 0; b < KC; ++b) {
-                    const f16x8 x = tr_pair(s_x, ax[b] + (kq * S + a) * H::PITCH * 128, 512);
+                    const f16x8 x = tr_pair(buf, ax[b] + (kq * S + a) * H::PITCH * 128, 512);
                     acc[a * KC + b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, gl, acc[a * KC + b], 0, 0, 0);
                     acc[a * KC + b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, gh, acc[a * KC + b], 0, 0, 0);
                 }
         }
+    };
+
+    if (tid < 2) s_flag[tid] = -1;
+    load(t0);
+    rescale();
+    expand(lds);
+    if (t0 + 1 < t1) load(t0 + 1);
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        unsigned char *now = lds + ((t - t0) & 1) * H::BUF, *next = lds + ((t - t0 + 1) & 1) * H::BUF;
+        const bool more = t + 1 < t1;
+        auto stage = [&]() {
+            if (!more) return;
+            const bool beyond = expand(next);
+            if (__any(beyond) && lane == 0) s_flag[(t + 1) & 1] = t + 1;
+            if (t + 2 < t1) load(t + 2);
+        };
+        if (TG == 1 || tg == 0) {
+            stage();
+            multiply(now);
+        } else {
+            multiply(now);
+            stage();
+        }
+        __syncthreads();
+        if (more && s_flag[(t + 1) & 1] == t + 1) {  // (the same for all: written before the barrier)
+            load(t + 1);
+            rescale();
+            expand(next);
+            if (t + 2 < t1) load(t + 2);
+            __syncthreads();
+        }
     }
-    const int cip = p.nci * 64, cop = p.nco * 64, back = ex - 140 + eg - 15;
+    const int cip = p.nci * 64, cop = p.nco * 64, back = ex - 135 + eg - 11;
+    const int tap0 = (grp * TG + tg) * KR * KC;
     float *dst = p.partial + (((long long)split * p.k * p.k + tap0) * cip + ci0 + 32 * wm) * cop + co0 + 32 * wn + (lane & 31);
 #pragma unroll
     for (int t = 0; t < KR * KC; ++t)
@@ -272,7 +310,7 @@ __global__ __launch_bounds__(NT) void wgrad8_reduce(const float *partial, int sp
 }
 
 struct Geo {
-    int kind, ry;  // 0: 3×3, 1: 4×4 stride 2, 2: 4×4 stride 1, 3: 8×8, 4: tap by tap
+    int kind;  // 0: 3×3, 1: 4×4 stride 2, 2: 4×4 stride 1, 3: 8×8, 4: tap by tap
     WgP p;
 };
 bool geometry(int64_t B, int32_t Hs, int32_t Ws, int32_t cin, int32_t MH, int32_t MW, int32_t cout, int32_t k,
@@ -284,21 +322,20 @@ bool geometry(int64_t B, int32_t Hs, int32_t Ws, int32_t cin, int32_t MH, int32_
     if (MH != (Hs + 2 * pad - k) / s + 1 || MW != (Ws + 2 * pad - k) / s + 1) return false;
     if (B > 0x7fffffffLL / ((int64_t)MH * MW) || B > 0x7fffffffLL / ((int64_t)Hs * Ws)) return false;
     g.kind = k == 3 && s == 1 ? 0 : k == 4 && s == 2 ? 1 : k == 4 && s == 1 ? 2 : k == 8 && s == 1 ? 3 : 4;
-    g.ry = g.kind == 1 ? 4 : 8;
     WgP &p = g.p;
     p = WgP{};
     p.B = (int)B; p.Hs = Hs; p.Ws = Ws; p.cin = cin; p.nb = (cin + 31) / 32; p.MH = MH; p.MW = MW; p.cout = cout;
     p.k = k; p.s = s; p.p = pad;
     p.nci = (cin + 63) / 64;
     p.nco = (cout + 63) / 64;
-    p.groups = g.kind == 0 ? 1 : g.kind <= 2 ? 2 : g.kind == 3 ? 8 : k * k;
-    p.tY = (MH + g.ry - 1) / g.ry;
+    p.groups = g.kind <= 1 ? 1 : g.kind == 2 ? 2 : g.kind == 3 ? 8 : k * k;
+    p.tY = (MH + 3) / 4;
     p.tX = (MW + 15) / 16;
     const long long tiles = B * p.tY * p.tX, work = (long long)p.nci * p.nco * p.groups;
     if (tiles > 0x7fffffffLL || work > (1 << 24)) return false;
     p.tiles = (int)tiles;
-    // two workgroups per CU, a K step each at least
-    const long long n = work >= 512 ? 1 : 512 / work;
+    // a workgroup for every place (two per CU, one of the eight-wave kind), a K step each at least
+    const long long places = g.kind == 1 ? 256 : 512, n = work >= places ? 1 : places / work;
     p.per_split = (int)((tiles + (n < tiles ? n : tiles) - 1) / (n < tiles ? n : tiles));
     p.splits = (p.tiles + p.per_split - 1) / p.per_split;
     return (long long)(p.splits + 7) / 8 * 8 * work <= 0x7fffffffLL;
@@ -325,11 +362,11 @@ extern "C" int esr_dconv_wgrad_act8(const int8_t *codes, const uint8_t *exps, in
     p.gvec = cout % 4 == 0 && (uintptr_t)dy % 16 == 0;
     const dim3 grid((unsigned)((p.splits + 7) / 8 * 8 * p.nci * p.nco * p.groups)), block(NT);
     switch (g.kind) {
-        case 0: hipLaunchKernelGGL((wgrad8_kernel<3, 3, 1, 8>), grid, block, 0, st, p); break;
-        case 1: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 2, 4>), grid, block, 0, st, p); break;
-        case 2: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 1, 8>), grid, block, 0, st, p); break;
-        case 3: hipLaunchKernelGGL((wgrad8_kernel<1, 8, 1, 8>), grid, block, 0, st, p); break;
-        default: hipLaunchKernelGGL((wgrad8_kernel<1, 1, 1, 8>), grid, block, 0, st, p);
+        case 0: hipLaunchKernelGGL((wgrad8_kernel<3, 3, 1, 1>), grid, block, 0, st, p); break;
+        case 1: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 2, 2>), grid, dim3(2 * NT), 0, st, p); break;
+        case 2: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 1, 1>), grid, block, 0, st, p); break;
+        case 3: hipLaunchKernelGGL((wgrad8_kernel<1, 8, 1, 1>), grid, block, 0, st, p); break;
+        default: hipLaunchKernelGGL((wgrad8_kernel<1, 1, 1, 1>), grid, block, 0, st, p);
     }
     hipLaunchKernelGGL(wgrad8_reduce, dim3((unsigned)((cout + 31) / 32) * cin * k * k), block, 0, st, p.partial, p.splits,
                        k * k, cin, cout, p.nci * 64, p.nco * 64, gw);
