@@ -31,7 +31,8 @@ def on(dev):
 
 
 def stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+    """The current stream's handle (without the Stream object that torch.cuda.current_stream makes: 0.3 us for 2)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def check_dev(what, *ts):
@@ -110,6 +111,7 @@ class Carrier(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x):
+        ctx.set_materialize_grads(False)  # a first-order backward has no gradient for it: not one of zeros either
         return torch.empty_strided(x.shape, (0,) * x.dim(), device=x.device, dtype=x.dtype)
 
     @staticmethod

@@ -300,3 +300,17 @@ def test_discriminator_with_checkpoints(gpu_device, norm):
     a, b = (_critic_step(nets[1], real, fake, rp, torch.float32, gpu_device) for _ in range(2))
     for p, q in zip(a, b):
         assert bool(p.isfinite().all()) and torch.equal(p, q)
+
+
+def test_carrier_adds_nothing_to_a_first_backward(gpu_device):
+    """The stand-in for x that a checkpointed layer saves passes no gradient of zeros on (a pass over x-sized memory and
+    an addition to the real one)."""
+    from torch.profiler import ProfilerActivity, profile
+    x = torch.randn(2, 64, 16, 16, device=gpu_device).contiguous(memory_format=torch.channels_last).requires_grad_()
+    y = gn.group_norm_lrelu(x, 32, checkpoint='int8')
+    gy = torch.randn_like(y)
+    torch.autograd.grad(y, x, gy, retain_graph=True)
+    with profile(activities=[ProfilerActivity.CPU]) as prof:
+        torch.autograd.grad(y, x, gy)
+    names = {e.name for e in prof.events()}
+    assert not names & {'aten::zeros', 'aten::fill_', 'aten::add', 'aten::add_', 'aten::copy_'}, names
