@@ -25,6 +25,8 @@
 
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int NT = 256;
 constexpr int MAXS = 256;   // row splits of a sample in a reduction
 constexpr int UN = 4;       // rows of a thread in flight
@@ -61,10 +63,11 @@ __device__ __forceinline__ void load_f(const float *src, long long i, float *v) 
         v[0] = src[i];
     }
 }
+// (non-temporal: what a pass writes does not push what the next one reads out of the 256 MB last-level cache)
 template <int V>
 __device__ __forceinline__ void store_f(float *dst, long long i, const float *v) {
-    if constexpr (V == 4) *reinterpret_cast<float4 *>(dst + i) = make_float4(v[0], v[1], v[2], v[3]);
-    else dst[i] = v[0];
+    if constexpr (V == 4) __builtin_nontemporal_store((f32x4){v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4 *>(dst + i));
+    else __builtin_nontemporal_store(v[0], dst + i);
 }
 // a row's raw input (values, or a word of codes and its exponent byte), loaded ahead of its use
 template <int V, bool Q8>
@@ -286,16 +289,15 @@ struct GnOut {
     uint8_t *exps, *yexps;
 };
 
-// The elementwise pass.  Workgroups go through samples and rows from the last to the first: what the reduction before
-// read last is still in the 256 MB last-level cache.  The first row block of the first sample also sums the parameter
-// gradients over the samples, in order.
+// The elementwise pass.  The first row block of the first sample also sums the parameter gradients over the samples, in
+// order.
 // BITS: MODE 1, 2: the input is in 8-bit blocks; MODE 0: blocks are written.
 template <int MODE, int V, bool BITS>
 __global__ __launch_bounds__(NT) void gn_apply(GnP p, GnOut o) {
     constexpr int UA = MODE == 2 ? 2 : UN;
     constexpr bool Q8 = MODE && BITS;
     const int tid = threadIdx.x, lane = tid % p.lanes, ph = tid / p.lanes;
-    const int n = p.N - 1 - (int)blockIdx.y, b = p.blocks - 1 - (int)blockIdx.x;
+    const int n = blockIdx.y, b = blockIdx.x;
     const int c = ((int)blockIdx.z * NT + lane) * V;
     const bool act = c < p.C;
     if (ph >= p.rpi) return;
