@@ -39,7 +39,6 @@ struct WgP {
     const float *dy;
     int B, Hs, Ws, cin, nb, MH, MW, cout, k, s, p, nci, nco, groups;
     int tY, tX, tiles, per_split, splits;  // K steps: rows and columns of tiles per image, all, per split
-    int xvec, gvec;                        // 16-code and float4 loads
     float *partial;                        // [splits][k·k][nci·64][nco·64]
 };
 
@@ -67,7 +66,9 @@ struct Shape {
     static constexpr int NX = (ROWS * COLS * 4 + NT - 1) / NT, NG = KPX * 16 / NT;
 };
 
-template <int KR, int KC, int S, int TG>
+// LV: how channels are loaded. 0: 16 codes and 4 gradients at once (cin a multiple of 16, cout of 4); 1: by fours; 2: one
+// by one.
+template <int KR, int KC, int S, int TG, int LV>
 __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
     using H = Shape<KR, KC, S, TG>;
     constexpr int RY = H::RY;
@@ -96,51 +97,78 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
         xr[j] = ry < H::ROWS && ci0 + 16 * (idx & 3) < p.cin ? ry << 16 | cx : -1;
         xd[j] = ry < H::ROWS ? (ry * H::PITCH + pos) * 128 + (((idx & 3) ^ (2 * ((pos >> 1) & 1))) << 5) : -1;
     }
-    uint4 rx[H::NX];
-    int re[H::NX];
+    // Every load is issued, from the tensor's first element where its place is outside, and its value dropped when it is
+    // expanded: no branch for which the loads in flight would have to be waited for.
+    uint32_t rx[H::NX][4];
+    int re[H::NX], ok = 0;
     f32x4 rg[H::NG];
     auto load = [&](int t) {
         const int img = t / (p.tY * p.tX), r = t - img * p.tY * p.tX, ty = r / p.tX;
         const int Y0 = ty * RY, X0 = (r - ty * p.tX) * 16;
         const int st = H::ONE ? p.s : 1, ys = Y0 * (H::ONE ? p.s : S) + oy, xs = X0 * (H::ONE ? p.s : S) + ox;
+        const long long pix0 = (long long)img * p.Hs * p.Ws;
+        const int8_t *codes = p.codes + pix0 * p.cin;
+        const uint8_t *exps = p.exps + pix0 * p.nb;
+        const float *dy = p.dy + (long long)img * p.MH * p.MW * p.cout;
+        ok = 0;
 #pragma unroll
         for (int j = 0; j < H::NX; ++j) {
-            const int sy = ys + (xr[j] >> 16) * st, sx = xs + (xr[j] & 0xffff) * st;
-            rx[j] = make_uint4(0, 0, 0, 0);
-            re[j] = 0;
-            if (xr[j] >= 0 && (unsigned)sy < (unsigned)p.Hs && (unsigned)sx < (unsigned)p.Ws) {
-                const int ci = ci0 + 16 * (tid & 3);
-                const long long pix = (img * p.Hs + sy) * p.Ws + sx;
-                const int8_t *c = p.codes + pix * p.cin + ci;
-                re[j] = p.exps[pix * p.nb + ci / act8::BLK];
-                if (p.xvec) {
-                    rx[j] = *reinterpret_cast<const uint4 *>(c);
-                } else {
-                    uint32_t q[4] = {0, 0, 0, 0};
-                    const int n = min(16, p.cin - ci);
+            const int sy = ys + (xr[j] >> 16) * st, sx = xs + (xr[j] & 0xffff) * st, ci = ci0 + 16 * (tid & 3);
+            const bool in = xr[j] >= 0 && (unsigned)sy < (unsigned)p.Hs && (unsigned)sx < (unsigned)p.Ws;
+            const unsigned pix = in ? sy * p.Ws + sx : 0, c = in ? ci : 0;
+            ok |= (int)in << j;
+            re[j] = exps[pix * (unsigned)p.nb + c / act8::BLK];
+            const int8_t *src = codes + (pix * (unsigned)p.cin + c);
+            if constexpr (LV == 0) {
+                const uint4 q = *reinterpret_cast<const uint4 *>(src);
+                rx[j][0] = q.x; rx[j][1] = q.y; rx[j][2] = q.z; rx[j][3] = q.w;
+            } else {
+                const int n = in ? p.cin - ci : 1;  // channels there are (>= 1)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (i < n) q[i >> 2] |= (uint32_t)(uint8_t)c[i] << (8 * (i & 3));
-                    rx[j] = make_uint4(q[0], q[1], q[2], q[3]);
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (LV == 1) {
+                        rx[j][i] = *reinterpret_cast<const uint32_t *>(src + (4 * i < n ? 4 * i : 0));
+                    } else {
+                        rx[j][i] = 0;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b)
+                            rx[j][i] |= (uint32_t)(uint8_t)src[4 * i + b < n ? 4 * i + b : 0] << (8 * b);
+                    }
                 }
             }
         }
 #pragma unroll
         for (int j = 0; j < H::NG; ++j) {
             const int idx = tid + j * H::NT, q = idx >> 4, co = co0 + 4 * (idx & 15), Y = Y0 + (q >> 4), X = X0 + (q & 15);
-            f32x4 v = {0.f, 0.f, 0.f, 0.f};
-            if (Y < p.MH && X < p.MW && co < p.cout) {
-                const float *g = p.dy + (long long)((img * p.MH + Y) * p.MW + X) * p.cout + co;
-                if (p.gvec) {
-                    v = *reinterpret_cast<const f32x4 *>(g);
-                } else {
+            const bool in = Y < p.MH && X < p.MW && co < p.cout;
+            const float *src = dy + (in ? (unsigned)(Y * p.MW + X) * (unsigned)p.cout + co : 0u);
+            ok |= (int)in << (16 + j);
+            if constexpr (LV < 2) {
+                rg[j] = *reinterpret_cast<const f32x4 *>(src);
+            } else {
+                const int n = in ? p.cout - co : 1;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (co + i < p.cout) v[i] = g[i];
-                }
+                for (int i = 0; i < 4; ++i) rg[j][i] = src[i < n ? i : 0];
             }
-            rg[j] = v;
         }
+    };
+    auto drop = [&]() {  // the values that are outside
+#pragma unroll
+        for (int j = 0; j < H::NX; ++j) {
+            const bool in = ok >> j & 1;
+            const int n = p.cin - ci0 - 16 * (tid & 3);
+            re[j] = in ? re[j] : 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (LV == 2) rx[j][i] &= n >= 4 * i + 4 ? ~0u : n <= 4 * i ? 0u : (1u << (8 * (n - 4 * i))) - 1;
+                rx[j][i] = in && (LV != 1 || 4 * i < n) ? rx[j][i] : 0;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < H::NG; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                rg[j][i] = (ok >> (16 + j) & 1) && (LV < 2 || co0 + 4 * (tid & 15) + i < p.cout) ? rg[j][i] : 0.f;
     };
 
     f32x16 acc[KR * KC];
@@ -153,6 +181,7 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
     // The loaded tile's largest exponent byte and |dy| (finite ones) over the workgroup; the scales raised to them.
     auto rescale = [&]() {
         unsigned me = 0, mg = 0;
+        drop();
 #pragma unroll
         for (int j = 0; j < H::NX; ++j) me = max(me, re[j] == 255 ? 0u : (unsigned)re[j]);
 #pragma unroll
@@ -185,17 +214,17 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
     // The loaded tile into an LDS tile; whether one of this thread's values is beyond the scales.
     auto expand = [&](unsigned char *buf) {
         int me = 0;
+        drop();
 #pragma unroll
         for (int j = 0; j < H::NX; ++j) {
             if (xd[j] < 0) break;
             me = max(me, re[j] == 255 ? 0 : re[j]);
             const _Float16 sc = re[j] == 255 ? (_Float16)__builtin_nanf("") : (_Float16)ldexpf(1.f, min(re[j] - ex, 2) + 3);
             const f16x2 s = {sc, sc}, off = s * (_Float16)-1152.f;
-            const uint32_t q[4] = {rx[j].x, rx[j].y, rx[j].z, rx[j].w};
             f16x2 o[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t u = q[i] ^ 0x80808080u;
+                const uint32_t u = rx[j][i] ^ 0x80808080u;
                 o[2 * i] = code_pair(u, 0x04010400u, s, off);
                 o[2 * i + 1] = code_pair(u, 0x04030402u, s, off);
             }
@@ -320,7 +349,8 @@ bool geometry(int64_t B, int32_t Hs, int32_t Ws, int32_t cin, int32_t MH, int32_
     if (k > 8 || Hs > 65535 || Ws > 65535 || pad > 8192 || s > 8192 || cin > 65536 || cout > 65536) return false;
     if (Hs + 2 * pad < k || Ws + 2 * pad < k) return false;
     if (MH != (Hs + 2 * pad - k) / s + 1 || MW != (Ws + 2 * pad - k) / s + 1) return false;
-    if (B > 0x7fffffffLL / ((int64_t)MH * MW) || B > 0x7fffffffLL / ((int64_t)Hs * Ws)) return false;
+    // (offsets within an image are 32-bit)
+    if ((int64_t)MH * MW > 0x7fffffffLL / cout / 4 || (int64_t)Hs * Ws > 0x7fffffffLL / cin || B > 0x7fffffff) return false;
     g.kind = k == 3 && s == 1 ? 0 : k == 4 && s == 2 ? 1 : k == 4 && s == 1 ? 2 : k == 8 && s == 1 ? 3 : 4;
     WgP &p = g.p;
     p = WgP{};
@@ -341,6 +371,19 @@ bool geometry(int64_t B, int32_t Hs, int32_t Ws, int32_t cin, int32_t MH, int32_
     return (long long)(p.splits + 7) / 8 * 8 * work <= 0x7fffffffLL;
 }
 
+template <int LV>
+void run(const Geo &g, hipStream_t st) {
+    const WgP &p = g.p;
+    const dim3 grid((unsigned)((p.splits + 7) / 8 * 8 * p.nci * p.nco * p.groups)), block(NT);
+    switch (g.kind) {
+        case 0: hipLaunchKernelGGL((wgrad8_kernel<3, 3, 1, 1, LV>), grid, block, 0, st, p); break;
+        case 1: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 2, 2, LV>), grid, dim3(2 * NT), 0, st, p); break;
+        case 2: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 1, 1, LV>), grid, block, 0, st, p); break;
+        case 3: hipLaunchKernelGGL((wgrad8_kernel<1, 8, 1, 1, LV>), grid, block, 0, st, p); break;
+        default: hipLaunchKernelGGL((wgrad8_kernel<1, 1, 1, 1, LV>), grid, block, 0, st, p);
+    }
+}
+
 }  // namespace
 
 extern "C" int64_t esr_dconv_wgrad_act8_workspace_bytes(int64_t B, int32_t Hs, int32_t Ws, int32_t cin, int32_t MH,
@@ -358,17 +401,12 @@ extern "C" int esr_dconv_wgrad_act8(const int8_t *codes, const uint8_t *exps, in
     const hipStream_t st = (hipStream_t)stream;
     WgP &p = g.p;
     p.codes = codes; p.exps = exps; p.dy = dy; p.partial = (float *)ws;
-    p.xvec = cin % 16 == 0 && (uintptr_t)codes % 16 == 0;
-    p.gvec = cout % 4 == 0 && (uintptr_t)dy % 16 == 0;
-    const dim3 grid((unsigned)((p.splits + 7) / 8 * 8 * p.nci * p.nco * p.groups)), block(NT);
-    switch (g.kind) {
-        case 0: hipLaunchKernelGGL((wgrad8_kernel<3, 3, 1, 1>), grid, block, 0, st, p); break;
-        case 1: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 2, 2>), grid, dim3(2 * NT), 0, st, p); break;
-        case 2: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 1, 1>), grid, block, 0, st, p); break;
-        case 3: hipLaunchKernelGGL((wgrad8_kernel<1, 8, 1, 1>), grid, block, 0, st, p); break;
-        default: hipLaunchKernelGGL((wgrad8_kernel<1, 1, 1, 1>), grid, block, 0, st, p);
-    }
-    hipLaunchKernelGGL(wgrad8_reduce, dim3((unsigned)((cout + 31) / 32) * cin * k * k), block, 0, st, p.partial, p.splits,
+    const bool v16 = cin % 16 == 0 && (uintptr_t)codes % 16 == 0, g4 = cout % 4 == 0 && (uintptr_t)dy % 16 == 0;
+    const int lv = v16 && g4 ? 0 : cin % 4 == 0 && (uintptr_t)codes % 4 == 0 && g4 ? 1 : 2;
+    if (lv == 0) run<0>(g, st);
+    else if (lv == 1) run<1>(g, st);
+    else run<2>(g, st);
+    hipLaunchKernelGGL(wgrad8_reduce, dim3((unsigned)((cout + 31) / 32) * cin * k * k), dim3(NT), 0, st, p.partial, p.splits,
                        k * k, cin, cout, p.nci * 64, p.nco * 64, gw);
     return hipGetLastError() == hipSuccess ? ESR_OK : ESR_ELAUNCH;
 }
