@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
         for (int j = 0; j < H::NX; ++j) {
             const int sy = ys + (xr[j] >> 16) * st, sx = xs + (xr[j] & 0xffff) * st, ci = ci0 + 16 * (tid & 3);
             const bool in = xr[j] >= 0 && (unsigned)sy < (unsigned)p.Hs && (unsigned)sx < (unsigned)p.Ws;
-            const unsigned pix = in ? sy * p.Ws + sx : 0, c = in ? ci : 0;
+            const unsigned m = -(unsigned)in, pix = (unsigned)(sy * p.Ws + sx) & m, c = (unsigned)ci & m;  // (no branch)
             ok |= (int)in << j;
             re[j] = exps[pix * (unsigned)p.nb + c / act8::BLK];
             const int8_t *src = codes + (pix * (unsigned)p.cin + c);
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
         for (int j = 0; j < H::NG; ++j) {
             const int idx = tid + j * H::NT, q = idx >> 4, co = co0 + 4 * (idx & 15), Y = Y0 + (q >> 4), X = X0 + (q & 15);
             const bool in = Y < p.MH && X < p.MW && co < p.cout;
-            const float *src = dy + (in ? (unsigned)(Y * p.MW + X) * (unsigned)p.cout + co : 0u);
+            const float *src = dy + (((unsigned)(Y * p.MW + X) * (unsigned)p.cout + co) & -(unsigned)in);
             ok |= (int)in << (16 + j);
             if constexpr (LV < 2) {
                 rg[j] = *reinterpret_cast<const f32x4 *>(src);
@@ -208,8 +208,8 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
         for (int q = 0; q < KR * KC; ++q)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[q][r] = ldexpf(acc[q][r], -down);
-        ex = ex2;
-        eg = eg2;
+        ex = __builtin_amdgcn_readfirstlane(ex2);
+        eg = __builtin_amdgcn_readfirstlane(eg2);
     };
     // The loaded tile into an LDS tile; whether one of this thread's values is beyond the scales.
     auto expand = [&](unsigned char *buf) {
@@ -281,6 +281,10 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
     rescale();
     expand(lds);
     if (t0 + 1 < t1) load(t0 + 1);
+    // (an int of unknown origin, once: where every value that meets in the loop's re[j] is a widened byte, the compiler
+    // carries bytes, widens them behind each load and so waits for the load where it is issued)
+#pragma unroll
+    for (int j = 0; j < H::NX; ++j) asm("" : "+v"(re[j]));
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
         unsigned char *now = lds + ((t - t0) & 1) * H::BUF, *next = lds + ((t - t0 + 1) & 1) * H::BUF;
@@ -317,24 +321,27 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
             dst[((long long)t * cip + (r & 3) + 8 * (r >> 2) + 4 * hl) * cop] = ldexpf(acc[t][r], back);
 }
 
-// gw[co][ci][t] = Σ over the splits: 32 consecutive co × 8 slices of the splits, a slice in order, then the slices
+// gw[co][ci][t] = Σ over the splits: 32 consecutive co (four to a thread) × 32 slices of the splits, a slice in order,
+// then the slices
 __global__ __launch_bounds__(NT) void wgrad8_reduce(const float *partial, int splits, int T, int cin, int cout, int cip,
                                                     int cop, float *gw) {
-    __shared__ float sl[8][32];
-    const int q = threadIdx.x >> 5, o = threadIdx.x & 31, nco = (cout + 31) / 32;
-    const int co = blockIdx.x % nco * 32 + o, row = blockIdx.x / nco, ci = row % cin, t = row / cin;
+    __shared__ f32x4 sl[32][8];
+    const int q = threadIdx.x >> 3, o = threadIdx.x & 7, nco = (cout + 31) / 32;
+    const int co = blockIdx.x % nco * 32, row = blockIdx.x / nco, ci = row % cin, t = row / cin;
     const long long step = (long long)T * cip * cop;
-    const float *src = partial + ((long long)t * cip + ci) * cop + co;
-    const int s0 = splits * q / 8, s1 = splits * (q + 1) / 8;
-    float v = 0.f;
-    if (co < cout)
+    const float *src = partial + ((long long)t * cip + ci) * cop + co + 4 * o;  // (cop is a multiple of 64)
+    const int s0 = splits * q / 32, s1 = splits * (q + 1) / 32;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-        for (int s = s0; s < s1; ++s) v += src[s * step];
+    for (int s = s0; s < s1; ++s) v += *reinterpret_cast<const f32x4 *>(src + s * step);
     sl[q][o] = v;
     __syncthreads();
-    if (q == 0 && co < cout) {
-        for (int r = 1; r < 8; ++r) v += sl[r][o];
-        gw[((long long)co * cin + ci) * T + t] = v;
+    if (threadIdx.x < 32 && co + (int)threadIdx.x < cout) {
+        const float *col = reinterpret_cast<const float *>(sl) + threadIdx.x;
+        float s = col[0];
+#pragma unroll
+        for (int r = 1; r < 32; ++r) s += col[32 * r];
+        gw[((long long)(co + threadIdx.x) * cin + ci) * T + t] = s;
     }
 }
 
