@@ -27,13 +27,18 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int NT = 256;
+constexpr int NT = 256, NTS = 1024;
+constexpr int SMALL_C = 256;  // channels of a chunk of gn_small, at most
 constexpr int MAXS = 256;   // row splits of a sample in a reduction
 constexpr int UN = 4;       // rows of a thread in flight
 
 // A thread holds V consecutive channels (V = 4: 16-byte accesses; V = 1 where C or a base is not a multiple of 4 values)
 // and walks rows; the 32 / V lanes of an 8-bit block sit side by side, a row takes `lanes` threads (its last block padded
-// to 32 channels) and a workgroup `rpi` rows at a time.  Rows wider than a workgroup are cut over blockIdx.z.
+// to 32 channels) and a workgroup `rpi` rows at a time.  Rows are cut into chunks of `step` channels over the grid: what a
+// workgroup has threads for, or (gn_small) the fewest whole groups and blocks.
+//
+// Three launches a pass: gn_sums over row splits, gn_finish per sample and set of groups, gn_apply.  Where a chunk of a
+// sample has few values, gn_small does the three steps of a pass in one workgroup of 1024 threads.
 struct GnP {
     const float *x;              // [N][HW][C], or null: codes / exps
     const int8_t *codes;
@@ -45,7 +50,7 @@ struct GnP {
     const double *grp;           // [N][G][8] per-group coefficients of the pass
     const double *sums, *sums_u; // [N][2][C]: s1, s2; [N][3][C]: Σu, Σu·x̂, Σu·gz
     long long HW;
-    int N, C, G, Cg, nb, lanes, rpi, chunks, splits, blocks;
+    int N, C, G, Cg, nb, lanes, rpi, step, chunks, splits, blocks;
     float slope, eps;
 };
 
@@ -89,44 +94,43 @@ struct Raw {
         else return v[k];
     }
 };
-// per-channel constants of a thread
+// per-channel constants of a thread; stat: the statistics from group g0 on of its sample
 template <int V>
 struct Chan {
     double mu[V], r[V], ga[V], be[V];
-    __device__ __forceinline__ void load(const GnP &p, int n, int c) {
+    __device__ __forceinline__ void load(const GnP &p, const double *stat, int g0, int c) {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const long long g = (long long)n * p.G + (c + k) / p.Cg;
-            mu[k] = p.stat[2 * g];
-            r[k] = p.stat[2 * g + 1];
+            const int g = (c + k) / p.Cg - g0;
+            mu[k] = stat[2 * g];
+            r[k] = stat[2 * g + 1];
             ga[k] = p.gamma ? (double)p.gamma[c + k] : 1.0;
             be[k] = p.beta ? (double)p.beta[c + k] : 0.0;
         }
     }
 };
 
-// partial[n][split][k][c]: MODE 0: Σd, Σd² (d = x − the group's first value); 1: Σgz, Σgz·x̂; 2: Σu, Σu·x̂, Σu·gz
-template <int MODE, int V, bool Q8>
-__global__ __launch_bounds__(NT) void gn_sums(GnP p, double *partial) {
+// groups of 32 channels, or one
+__host__ __device__ __forceinline__ int sets(int Cg) { return Cg <= 32 ? 32 / Cg : 1; }
+
+// Sums over rows r0 .. r1 of a sample's chunk, each handed to put(k, channel, sum): MODE 0: Σd, Σd² (d = x − the group's
+// first value); 1: Σgz, Σgz·x̂; 2: Σu, Σu·x̂, Σu·gz.  ch: the thread's channels (MODE 1, 2).
+template <int MODE, int V, bool Q8, int NT, typename F>
+__device__ __forceinline__ void sums_of(const GnP &p, const Chan<V> &ch, int n, int chunk, long long r0, long long r1, F put) {
     constexpr int K = MODE == 2 ? 3 : 2;
     __shared__ double red[K * V][NT];
-    const int tid = threadIdx.x, lane = tid % p.lanes, ph = tid / p.lanes, n = blockIdx.y, sp = blockIdx.x;
-    const int c = ((int)blockIdx.z * NT + lane) * V;
-    const long long r0 = p.HW * sp / p.splits, r1 = p.HW * (sp + 1) / p.splits;
+    const int tid = threadIdx.x, lane = tid % p.lanes, ph = tid / p.lanes;
+    const int c = chunk * p.step + lane * V, c1 = min(p.C, (chunk + 1) * p.step);
     double s[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int v = 0; v < V; ++v) s[k][v] = 0.0;
-    if (ph < p.rpi && c < p.C) {
-        Chan<V> ch;
+    if (ph < p.rpi && c < c1) {
         double pivot[V];
-        if constexpr (MODE == 0) {
+        if constexpr (MODE == 0)
 #pragma unroll
             for (int v = 0; v < V; ++v) pivot[v] = p.x[(long long)n * p.HW * p.C + (c + v) / p.Cg * p.Cg];
-        } else {
-            ch.load(p, n, c);
-        }
         for (long long q = r0 + ph; q < r1; q += UN * p.rpi) {
             Raw<V, Q8> raw[UN];
             float gy[UN][V], u[UN][V];
@@ -163,70 +167,113 @@ __global__ __launch_bounds__(NT) void gn_sums(GnP p, double *partial) {
             }
         }
     }
+    // the rows of a workgroup, in a fixed order: those of a wave by lane exchanges where a row's lanes divide it, then the
+    // waves' (or all rows') through LDS
+    const bool fold = p.lanes < 64 && (p.lanes & (p.lanes - 1)) == 0;
+    const int parts = fold ? NT / 64 : p.rpi, at = fold ? (tid >> 6) * p.lanes + lane : tid;
+    if (fold)
+        for (int d = p.lanes; d < 64; d <<= 1)
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+            for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int v = 0; v < V; ++v) red[k * V + v][tid] = s[k][v];
+                for (int v = 0; v < V; ++v) s[k][v] += __shfl_xor(s[k][v], d);
+    if (!fold || (tid & 63) < p.lanes)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) red[k * V + v][at] = s[k][v];
     __syncthreads();
-    for (int i = tid; i < K * V * p.lanes; i += NT) {  // the rows of a workgroup, in order
-        const int ln = i / V % p.lanes, k = i / V / p.lanes, v = i % V;
-        const int cc = ((int)blockIdx.z * NT + ln) * V + v;
-        if (cc >= p.C) continue;
-        double t = red[k * V + v][ln];
-        for (int q = 1; q < p.rpi; ++q) t += red[k * V + v][q * p.lanes + ln];
-        partial[(((long long)n * p.splits + sp) * K + k) * p.C + cc] = t;
+    for (int i = tid; i < K * V * p.lanes; i += NT) {
+        const int ln = i % p.lanes, kv = i / p.lanes, cc = chunk * p.step + ln * V + kv % V;
+        if (cc >= c1) continue;
+        double t = red[kv][ln];
+#pragma unroll 4
+        for (int q = 1; q < parts; ++q) t += red[kv][q * p.lanes + ln];
+        put(kv / V, cc, t);
     }
 }
 
-// One workgroup per sample and set of whole groups (32 channels' worth, or one larger group): the splits' sums per
-// channel (sums_out [n][K][C], or null), then each group's: MODE 0: out = μ, r; 1: S1/M, S2/M; 2: the seven coefficients
-// of the double backward (partial null: no upstream of gx).
+// A group's share of channel c, from its sums s: MODE 0, 1: s0, s1 (times γ); 2: S1, S2, U, A, Q, Σ ga·s1, Σ ga·s2
+template <int MODE>
+__device__ __forceinline__ void shares(const GnP &p, int n, int c, const double *s, double *out) {
+    const double ga = MODE && p.gamma ? (double)p.gamma[c] : 1.0;
+    if constexpr (MODE < 2) {
+        out[0] = ga * s[0];
+        out[1] = ga * s[1];
+    } else {
+        const double s1 = p.sums[(long long)n * 2 * p.C + c], s2 = p.sums[((long long)n * 2 + 1) * p.C + c];
+        const double a = p.gga ? (double)p.gga[c] : 0.0;
+        out[0] = ga * s1;
+        out[1] = ga * s2;
+        out[2] = s[0];
+        out[3] = s[1];
+        out[4] = ga * s[2];
+        out[5] = p.gga ? a * s1 : 0.0;
+        out[6] = p.gga ? a * s2 : 0.0;
+    }
+}
+// A group's results from the totals of its shares: MODE 0: μ, r; 1: S1/M, S2/M; 2: the seven coefficients of the double
+// backward
+template <int MODE>
+__device__ __forceinline__ void results(const GnP &p, int n, int g, const double *t, double *out) {
+    const double M = (double)p.HW * p.Cg, t0 = t[0] / M, t1 = t[1] / M;
+    if constexpr (MODE == 0) {
+        const double var0 = t1 - t0 * t0, var = var0 < 0.0 ? 0.0 : var0;  // (a NaN stays one)
+        out[0] = p.x[(long long)n * p.HW * p.C + g * p.Cg] + t0;
+        out[1] = 1.0 / sqrt(var + (double)p.eps);
+    } else if constexpr (MODE == 1) {
+        out[0] = t0;
+        out[1] = t1;
+    } else {
+        const double r = p.stat[2 * ((long long)n * p.G + g) + 1], u = t[2] / M, a = t[3] / M;
+        out[0] = u;
+        out[1] = a;
+        out[2] = t0;
+        out[3] = t1;
+        out[4] = -r * (t0 * a + u * t1) + t[5] / M;
+        out[5] = -2.0 * r * t1 * a + t[6] / M;
+        out[6] = (t[4] / M - t0 * u - t1 * a) * r * r;
+    }
+}
+template <int MODE>
+struct Sizes {
+    static constexpr int K = MODE == 2 ? 3 : 2, J = MODE == 2 ? 7 : 2, O = MODE ? 8 : 2;  // sums, shares, results
+};
+
+// A workgroup per sample and set of whole groups (32 channels' worth, or one larger group): the splits' sums per channel
+// (sums_out [n][K][C], or null), then each group's results (partial null: no upstream of gx).
 template <int MODE>
 __global__ __launch_bounds__(NT) void gn_finish(GnP p, const double *partial, double *sums_out, double *out) {
-    constexpr int K = MODE == 2 ? 3 : 2, J = MODE == 2 ? 7 : 2;
-    __shared__ double part[8][K][32], chan[J][33], tot[J][32];
+    using S = Sizes<MODE>;
+    __shared__ double part[8][S::K][32], chan[S::J][33], tot[S::J][32];
     const int tid = threadIdx.x, lane = tid & 31, sl = tid >> 5, n = blockIdx.y;
-    const int gpb = p.Cg <= 32 ? 32 / p.Cg : 1, g0 = blockIdx.x * gpb, ng = min(gpb, p.G - g0);
-    const int c1 = (g0 + ng) * p.Cg;
-    for (int i = tid; i < J * 32; i += NT) tot[i / 32][i % 32] = 0.0;
+    const int gpb = sets(p.Cg), g0 = blockIdx.x * gpb, ng = min(gpb, p.G - g0), c1 = (g0 + ng) * p.Cg;
+    for (int i = tid; i < S::J * 32; i += NT) tot[i / 32][i % 32] = 0.0;
     for (int c0 = g0 * p.Cg; c0 < c1; c0 += 32) {
         const int c = c0 + lane;
-        double s[K] = {};
+        double s[S::K] = {};
         if (c < c1 && partial)
 #pragma unroll 4
             for (int sp = sl; sp < p.splits; sp += 8)
 #pragma unroll
-                for (int k = 0; k < K; ++k) s[k] += partial[(((long long)n * p.splits + sp) * K + k) * p.C + c];
+                for (int k = 0; k < S::K; ++k) s[k] += partial[(((long long)n * p.splits + sp) * S::K + k) * p.C + c];
 #pragma unroll
-        for (int k = 0; k < K; ++k) part[sl][k][lane] = s[k];
+        for (int k = 0; k < S::K; ++k) part[sl][k][lane] = s[k];
         __syncthreads();
-        if (sl == 0) {
+        if (sl == 0 && c < c1) {
+            double sh[S::J];
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
+            for (int k = 0; k < S::K; ++k) {
                 s[k] = part[0][k][lane];
                 for (int q = 1; q < 8; ++q) s[k] += part[q][k][lane];
-                if (sums_out && c < c1) sums_out[((long long)n * K + k) * p.C + c] = s[k];
+                if (sums_out) sums_out[((long long)n * S::K + k) * p.C + c] = s[k];
             }
-            const double ga = MODE && p.gamma && c < c1 ? (double)p.gamma[c] : 1.0;
-            if constexpr (MODE < 2) {
-                chan[0][lane] = ga * s[0];
-                chan[1][lane] = ga * s[1];
-            } else {
-                const bool in = c < c1;
-                const double s1 = in ? p.sums[(long long)n * 2 * p.C + c] : 0.0;
-                const double s2 = in ? p.sums[((long long)n * 2 + 1) * p.C + c] : 0.0;
-                const double a = in && p.gga ? (double)p.gga[c] : 0.0;
-                chan[0][lane] = ga * s1;
-                chan[1][lane] = ga * s2;
-                chan[2][lane] = s[0];
-                chan[3][lane] = s[1];
-                chan[4][lane] = ga * s[K - 1];
-                chan[5][lane] = p.gga ? a * s1 : 0.0;
-                chan[6][lane] = p.gga ? a * s2 : 0.0;
-            }
+            shares<MODE>(p, n, c, s, sh);
+#pragma unroll
+            for (int j = 0; j < S::J; ++j) chan[j][lane] = sh[j];
         }
         __syncthreads();
-        for (int i = tid; i < J * ng; i += NT) {  // channels of a group, in order
+        for (int i = tid; i < S::J * ng; i += NT) {  // channels of a group, in order
             const int j = i / ng, g = i - j * ng, a = p.Cg <= 32 ? g * p.Cg : 0;
             const int b = p.Cg <= 32 ? a + p.Cg : min(32, c1 - c0);
             double t = tot[j][g];
@@ -236,25 +283,10 @@ __global__ __launch_bounds__(NT) void gn_finish(GnP p, const double *partial, do
         __syncthreads();
     }
     if (tid >= ng) return;
-    const long long i = (long long)n * p.G + g0 + tid;
-    const double M = (double)p.HW * p.Cg, t0 = tot[0][tid] / M, t1 = tot[1][tid] / M;
-    if constexpr (MODE == 0) {
-        const double var0 = t1 - t0 * t0, var = var0 < 0.0 ? 0.0 : var0;  // (a NaN stays one)
-        out[2 * i] = p.x[(long long)n * p.HW * p.C + (g0 + tid) * p.Cg] + t0;
-        out[2 * i + 1] = 1.0 / sqrt(var + (double)p.eps);
-    } else if constexpr (MODE == 1) {
-        out[8 * i] = t0;
-        out[8 * i + 1] = t1;
-    } else {
-        const double r = p.stat[2 * i + 1], u = tot[J - 5][tid] / M, a = tot[J - 4][tid] / M;
-        out[8 * i] = u;
-        out[8 * i + 1] = a;
-        out[8 * i + 2] = t0;
-        out[8 * i + 3] = t1;
-        out[8 * i + 4] = -r * (t0 * a + u * t1) + tot[J - 2][tid] / M;
-        out[8 * i + 5] = -2.0 * r * t1 * a + tot[J - 1][tid] / M;
-        out[8 * i + 6] = (tot[J - 3][tid] / M - t0 * u - t1 * a) * r * r;
-    }
+    double t[S::J];
+#pragma unroll
+    for (int j = 0; j < S::J; ++j) t[j] = tot[j][tid];
+    results<MODE>(p, n, g0 + tid, t, out + S::O * ((long long)n * p.G + g0 + tid));
 }
 
 // codes of V values of one row in a block whose lanes call together; pre: z of a value
@@ -289,45 +321,42 @@ struct GnOut {
     uint8_t *exps, *yexps;
 };
 
-// The elementwise pass.  The first row block of the first sample also sums the parameter gradients over the samples, in
-// order.
+// dγ and dβ (MODE 1) or g_γ (MODE 2) of a channel: sums over the samples, in order
+template <int MODE>
+__device__ __forceinline__ void params_of(const GnP &p, int c, float *g_gamma, float *g_beta) {
+    double s = 0.0, t = 0.0;
+    for (int i = 0; i < p.N; ++i) {
+        const double *q = p.sums + (long long)i * 2 * p.C + c;
+        if constexpr (MODE == 1) {
+            s += q[p.C];
+            t += q[0];
+        } else if (p.sums_u) {
+            const long long g = (long long)i * p.G + c / p.Cg;
+            s += p.stat[2 * g + 1] * (p.sums_u[((long long)i * 3 + 2) * p.C + c] - q[0] * p.grp[8 * g] -
+                                      q[p.C] * p.grp[8 * g + 1]);
+        }
+    }
+    if (g_gamma) g_gamma[c] = (float)s;
+    if (MODE == 1 && g_beta) g_beta[c] = (float)t;
+}
+
+// The elementwise pass over rows r0 .. r1 of a sample's chunk; grp: the coefficients from group g0 on of the sample.
 // BITS: MODE 1, 2: the input is in 8-bit blocks; MODE 0: blocks are written.
 template <int MODE, int V, bool BITS>
-__global__ __launch_bounds__(NT) void gn_apply(GnP p, GnOut o) {
+__device__ __forceinline__ void apply_of(const GnP &p, const GnOut &o, const Chan<V> &ch, const double *grp, int g0, int n,
+                                         int chunk, long long r0, long long r1) {
     constexpr int UA = MODE == 2 ? 2 : UN;
     constexpr bool Q8 = MODE && BITS;
     const int tid = threadIdx.x, lane = tid % p.lanes, ph = tid / p.lanes;
-    const int n = blockIdx.y, b = blockIdx.x;
-    const int c = ((int)blockIdx.z * NT + lane) * V;
-    const bool act = c < p.C;
+    const int c = chunk * p.step + lane * V;
+    const bool act = c < min(p.C, (chunk + 1) * p.step);
     if (ph >= p.rpi) return;
-    if (MODE && b == 0 && n == 0 && ph == 0 && act) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            double s = 0.0, t = 0.0;
-            for (int i = 0; i < p.N; ++i) {
-                const double *q = p.sums + (long long)i * 2 * p.C + c + v;
-                if constexpr (MODE == 1) {
-                    s += q[p.C];
-                    t += q[0];
-                } else if (p.sums_u) {
-                    const long long g = (long long)i * p.G + (c + v) / p.Cg;
-                    s += p.stat[2 * g + 1] * (p.sums_u[((long long)i * 3 + 2) * p.C + c + v] - q[0] * p.grp[8 * g] -
-                                              q[p.C] * p.grp[8 * g + 1]);
-                }
-            }
-            if (o.g_gamma) o.g_gamma[c + v] = (float)s;
-            if (MODE == 1 && o.g_beta) o.g_beta[c + v] = (float)t;
-        }
-    }
-    Chan<V> ch;
     float k0[V], k1[V], k3[V], k4[V], k5[V], k6[V], ua[V], ub[V];
     if (act) {
-        ch.load(p, n, c);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             if constexpr (MODE >= 1) {
-                const double *k = p.grp + 8 * ((long long)n * p.G + (c + v) / p.Cg);
+                const double *k = grp + 8 * ((c + v) / p.Cg - g0);
                 k0[v] = (float)k[0];
                 k1[v] = (float)k[1];
                 if constexpr (MODE == 2) {
@@ -341,7 +370,6 @@ __global__ __launch_bounds__(NT) void gn_apply(GnP p, GnOut o) {
             }
         }
     }
-    const long long r0 = p.HW * b / p.blocks, r1 = p.HW * (b + 1) / p.blocks;
     for (long long q = r0 + ph; q < r1; q += UA * p.rpi) {
         Raw<V, Q8> raw[UA];
         float gy[UA][V], u[UA][V];
@@ -403,6 +431,79 @@ __global__ __launch_bounds__(NT) void gn_apply(GnP p, GnOut o) {
     }
 }
 
+template <int MODE, int V, bool Q8>
+__global__ __launch_bounds__(NT) void gn_sums(GnP p, double *partial) {
+    constexpr int K = Sizes<MODE>::K;
+    const int sp = blockIdx.x, n = blockIdx.y, chunk = blockIdx.z, c = chunk * p.step + (int)threadIdx.x % p.lanes * V;
+    Chan<V> ch;
+    if constexpr (MODE > 0)
+        if (c < p.C) ch.load(p, p.stat + 2LL * n * p.G, 0, c);
+    sums_of<MODE, V, Q8, NT>(p, ch, n, chunk, p.HW * sp / p.splits, p.HW * (sp + 1) / p.splits, [&](int k, int cc, double s) {
+        partial[(((long long)n * p.splits + sp) * K + k) * p.C + cc] = s;
+    });
+}
+// (the first row block of the first sample also makes the parameter gradients)
+template <int MODE, int V, bool BITS>
+__global__ __launch_bounds__(NT) void gn_apply(GnP p, GnOut o) {
+    const int b = blockIdx.x, n = blockIdx.y, chunk = blockIdx.z, c = chunk * p.step + (int)threadIdx.x % p.lanes * V;
+    if constexpr (MODE > 0)
+        if (b == 0 && n == 0)
+            for (int i = chunk * p.step + threadIdx.x; i < min(p.C, (chunk + 1) * p.step); i += NT)
+                params_of<MODE>(p, i, o.g_gamma, o.g_beta);
+    Chan<V> ch;
+    if (c < p.C) ch.load(p, p.stat + 2LL * n * p.G, 0, c);
+    apply_of<MODE, V, BITS>(p, o, ch, p.grp + 8LL * n * p.G, 0, n, chunk, p.HW * b / p.blocks, p.HW * (b + 1) / p.blocks);
+}
+// A whole pass of one sample's chunk, sums and coefficients in LDS (and in memory what a later launch reads).
+template <int MODE, int V, bool BITS>
+__global__ __launch_bounds__(NTS) void gn_small(GnP p, GnOut o, double *sums_out, double *out) {
+    using S = Sizes<MODE>;
+    __shared__ double s_sum[S::K][SMALL_C], s_out[SMALL_C][S::O];
+    const int n = blockIdx.y, chunk = blockIdx.x, c0 = chunk * p.step, c1 = min(p.C, c0 + p.step), g0 = c0 / p.Cg;
+    const int tid = threadIdx.x, c = c0 + tid % p.lanes * V;
+    Chan<V> ch;
+    if constexpr (MODE > 0)
+        if (c < c1) ch.load(p, p.stat + 2LL * n * p.G, 0, c);
+    if (MODE < 2 || p.u) {
+        sums_of<MODE, V, MODE && BITS, NTS>(p, ch, n, chunk, 0, p.HW, [&](int k, int cc, double s) {
+            s_sum[k][cc - c0] = s;
+            if (sums_out) sums_out[((long long)n * S::K + k) * p.C + cc] = s;
+        });
+    } else {
+        for (int i = tid; i < S::K * SMALL_C; i += NTS) s_sum[i / SMALL_C][i % SMALL_C] = 0.0;
+    }
+    __syncthreads();
+    if (tid < (c1 - c0) / p.Cg) {
+        const int g = g0 + tid;
+        double t[S::J] = {}, sh[S::J], s[S::K], res[S::O] = {};
+        for (int i = g * p.Cg; i < (g + 1) * p.Cg; ++i) {  // channels of a group, in order
+#pragma unroll
+            for (int k = 0; k < S::K; ++k) s[k] = s_sum[k][i - c0];
+            shares<MODE>(p, n, i, s, sh);
+#pragma unroll
+            for (int j = 0; j < S::J; ++j) t[j] += sh[j];
+        }
+        results<MODE>(p, n, g, t, res);
+#pragma unroll
+        for (int j = 0; j < S::O; ++j) {
+            s_out[tid][j] = res[j];
+            out[S::O * ((long long)n * p.G + g) + j] = res[j];
+        }
+    }
+    __syncthreads();
+    if constexpr (MODE > 0)
+        if (p.N == 1)  // its sums and coefficients are this workgroup's own
+            for (int i = c0 + tid; i < c1; i += NTS) params_of<MODE>(p, i, o.g_gamma, o.g_beta);
+    if constexpr (MODE == 0)
+        if (c < c1) ch.load(p, &s_out[0][0], g0, c);
+    apply_of<MODE, V, BITS>(p, o, ch, &s_out[0][0], g0, n, chunk, 0, p.HW);
+}
+template <int MODE>
+__global__ void gn_params(GnP p, float *g_gamma, float *g_beta) {
+    const int c = blockIdx.x * NT + threadIdx.x;
+    if (c < p.C) params_of<MODE>(p, c, g_gamma, g_beta);
+}
+
 inline int launched() { return hipGetLastError() == hipSuccess ? ESR_OK : ESR_ELAUNCH; }
 
 inline bool shape_ok(int64_t N, int64_t HW, int32_t C, int32_t G) {
@@ -421,15 +522,32 @@ inline bool aligned(std::initializer_list<const void *> f32, std::initializer_li
     return true;
 }
 
+// the fewest channels of whole groups and, unless it is all of them, whole 8-bit blocks
+int chunk_of(int32_t C, int32_t Cg) {
+    int64_t s = Cg;
+    while (s % act8::BLK) s += Cg;  // at most 32 times
+    return s < C ? (int)s : C;
+}
+
 GnP params(int V, int64_t N, int64_t HW, int32_t C, int32_t G, const float *gamma, const float *beta, float slope) {
     GnP p{};
     p.gamma = gamma; p.beta = beta;
     p.N = (int)N; p.HW = HW; p.C = C; p.G = G; p.Cg = C / G; p.slope = slope;
     p.nb = (C + act8::BLK - 1) / act8::BLK;
-    const int lanes = p.nb * (act8::BLK / V);
-    p.chunks = (lanes + NT - 1) / NT;
-    p.lanes = lanes < NT ? lanes : NT;
-    p.rpi = NT / p.lanes;
+    // One workgroup per sample and chunk where that is at most 128 K values: 4 us for 3×40×36×64 against 17 us in three
+    // launches, break-even at twice the limit.
+    const int small = chunk_of(C, p.Cg), ln = (small + act8::BLK - 1) / act8::BLK * (act8::BLK / V);
+    const bool one = small <= SMALL_C && HW <= (128 << 10) / small;
+    const int threads = one ? NTS : NT, lanes = one ? ln : p.nb * (act8::BLK / V);
+    p.lanes = lanes < threads ? lanes : threads;
+    p.step = one ? small : p.lanes * V;
+    p.chunks = (C + p.step - 1) / p.step;
+    p.rpi = threads / p.lanes;
+    if (one) {
+        p.splits = 1;
+        p.blocks = 0;
+        return p;
+    }
     // ~4 workgroups per CU for the sums (each leaves K·C float64 partials), 8 for the elementwise pass, of at least UN
     // rows per thread
     const int64_t per = (int64_t)N * p.chunks, rows = (HW + UN * p.rpi - 1) / (UN * p.rpi);
@@ -443,22 +561,34 @@ GnP params(int V, int64_t N, int64_t HW, int32_t C, int32_t G, const float *gamm
     return p;
 }
 
-template <int MODE, bool Q8>
-void sums(const GnP &p, int V, double *partial, hipStream_t st) {
-    const dim3 grid(p.splits, p.N, p.chunks);
-    if (V == 4) hipLaunchKernelGGL((gn_sums<MODE, 4, Q8>), grid, dim3(NT), 0, st, p, partial);
-    else hipLaunchKernelGGL((gn_sums<MODE, 1, Q8>), grid, dim3(NT), 0, st, p, partial);
+// The launches of a pass: sums_out gets the reduction's sums (null: not wanted), out the statistics (MODE 0) or the
+// groups' coefficients.
+template <int MODE, int V, bool BITS>
+void pass(GnP p, const GnOut &o, double *partial, double *sums_out, double *out, hipStream_t st) {
+    if constexpr (MODE == 0) p.stat = out;
+    else p.grp = out;
+    if constexpr (MODE == 1) p.sums = sums_out;
+    if constexpr (MODE == 2) p.sums_u = p.u ? sums_out : nullptr;
+    if (!p.blocks) {
+        hipLaunchKernelGGL((gn_small<MODE, V, BITS>), dim3(p.chunks, p.N), dim3(NTS), 0, st, p, o, sums_out, out);
+        if (MODE && p.N > 1 && (o.g_gamma || o.g_beta))
+            hipLaunchKernelGGL(gn_params<MODE>, dim3((p.C + NT - 1) / NT), dim3(NT), 0, st, p, o.g_gamma, o.g_beta);
+        return;
+    }
+    const bool reduce = MODE < 2 || p.u;
+    const int gpb = sets(p.Cg);
+    if (reduce)
+        hipLaunchKernelGGL((gn_sums<MODE, V, MODE && BITS>), dim3(p.splits, p.N, p.chunks), dim3(NT), 0, st, p, partial);
+    hipLaunchKernelGGL(gn_finish<MODE>, dim3((p.G + gpb - 1) / gpb, p.N), dim3(NT), 0, st, p, reduce ? partial : nullptr,
+                       sums_out, out);
+    hipLaunchKernelGGL((gn_apply<MODE, V, BITS>), dim3(p.blocks, p.N, p.chunks), dim3(NT), 0, st, p, o);
 }
 template <int MODE>
-void finish(const GnP &p, const double *partial, double *sums_out, double *out, hipStream_t st) {
-    const int gpb = p.Cg <= 32 ? 32 / p.Cg : 1;
-    hipLaunchKernelGGL(gn_finish<MODE>, dim3((p.G + gpb - 1) / gpb, p.N), dim3(NT), 0, st, p, partial, sums_out, out);
-}
-template <int MODE, bool BITS>
-void apply(const GnP &p, int V, const GnOut &o, hipStream_t st) {
-    const dim3 grid(p.blocks, p.N, p.chunks);
-    if (V == 4) hipLaunchKernelGGL((gn_apply<MODE, 4, BITS>), grid, dim3(NT), 0, st, p, o);
-    else hipLaunchKernelGGL((gn_apply<MODE, 1, BITS>), grid, dim3(NT), 0, st, p, o);
+void pass(const GnP &p, int V, bool bits, const GnOut &o, double *partial, double *sums_out, double *out, hipStream_t st) {
+    if (V == 4 && bits) pass<MODE, 4, true>(p, o, partial, sums_out, out, st);
+    else if (V == 4) pass<MODE, 4, false>(p, o, partial, sums_out, out, st);
+    else if (bits) pass<MODE, 1, true>(p, o, partial, sums_out, out, st);
+    else pass<MODE, 1, false>(p, o, partial, sums_out, out, st);
 }
 
 }  // namespace
@@ -480,13 +610,8 @@ extern "C" int esr_gn_lrelu_fwd(const float *x, int64_t N, int64_t HW, int32_t C
     const int V = C % 4 == 0 && aligned({x, y}, {codes, ycodes}) ? 4 : 1;
     GnP p = params(V, N, HW, C, G, gamma, beta, slope);
     p.x = x; p.eps = eps;
-    double *partial = (double *)ws;
-    sums<0, false>(p, V, partial, st);
-    finish<0>(p, partial, nullptr, stat, st);
-    p.stat = stat;
-    const GnOut o{y, nullptr, nullptr, nullptr, codes, ycodes, exps, yexps};
-    if (codes || ycodes) apply<0, true>(p, V, o, st);
-    else apply<0, false>(p, V, o, st);
+    pass<0>(p, V, codes || ycodes, GnOut{y, nullptr, nullptr, nullptr, codes, ycodes, exps, yexps}, (double *)ws, nullptr,
+            stat, st);
     return launched();
 }
 
@@ -500,13 +625,7 @@ extern "C" int esr_gn_lrelu_bwd(const float *x, const int8_t *codes, const uint8
     GnP p = params(V, N, HW, C, G, gamma, beta, slope);
     p.x = x; p.codes = codes; p.exps = exps; p.gy = gy; p.stat = stat;
     double *partial = (double *)ws, *grp = partial + N * p.splits * 3 * C + N * 3 * C;
-    if (x) sums<1, false>(p, V, partial, st);
-    else sums<1, true>(p, V, partial, st);
-    finish<1>(p, partial, sums_, grp, st);
-    p.grp = grp; p.sums = sums_;
-    const GnOut o{gx, nullptr, g_gamma, g_beta, nullptr, nullptr, nullptr, nullptr};
-    if (x) apply<1, false>(p, V, o, st);
-    else apply<1, true>(p, V, o, st);
+    pass<1>(p, V, !x, GnOut{gx, nullptr, g_gamma, g_beta, nullptr, nullptr, nullptr, nullptr}, partial, sums_, grp, st);
     return launched();
 }
 
@@ -523,14 +642,6 @@ extern "C" int esr_gn_lrelu_bwd2(const float *x, const int8_t *codes, const uint
     p.x = x; p.codes = codes; p.exps = exps; p.gy = gy; p.u = u; p.gga = gg_gamma; p.ggb = gg_beta; p.stat = stat;
     p.sums = sums_;
     double *partial = (double *)ws, *su = partial + N * p.splits * 3 * C, *grp = su + N * 3 * C;
-    if (u) {
-        if (x) sums<2, false>(p, V, partial, st);
-        else sums<2, true>(p, V, partial, st);
-    }
-    finish<2>(p, u ? partial : nullptr, su, grp, st);
-    p.grp = grp; p.sums_u = u ? su : nullptr;
-    const GnOut o{g_x, g_gy, g_gamma, nullptr, nullptr, nullptr, nullptr, nullptr};
-    if (x) apply<2, false>(p, V, o, st);
-    else apply<2, true>(p, V, o, st);
+    pass<2>(p, V, !x, GnOut{g_x, g_gy, g_gamma, nullptr, nullptr, nullptr, nullptr, nullptr}, partial, su, grp, st);
     return launched();
 }

@@ -18,7 +18,10 @@ pytestmark = pytest.mark.gpu
 # width divides, more channels than a workgroup has threads, odd maps, several row splits
 SHAPES = [((1, 1, 1, 1), 1), ((1, 4, 1, 1), 2), ((2, 3, 5, 7), 3), ((3, 100, 9, 7), 4), ((2, 64, 13, 11), 32),
           ((1, 512, 3, 5), 32), ((2, 37, 6, 5), 1), ((5, 256, 4, 4), 256), ((1, 1025, 2, 3), 25), ((1, 1300, 3, 2), 13),
-          ((2, 96, 33, 3), 32), ((1, 64, 70, 65), 8), ((4, 128, 20, 18), 1), ((2, 33, 17, 2), 11), ((33, 8, 2, 2), 4)]
+          ((2, 96, 33, 3), 32), ((1, 64, 70, 65), 8), ((4, 128, 20, 18), 1), ((2, 33, 17, 2), 11), ((33, 8, 2, 2), 4),
+          # chunks of lcm(channels of a group, 32) channels; a sample too large for one workgroup and just not
+          ((2, 288, 5, 6), 96), ((1, 320, 4, 7), 20), ((3, 192, 9, 2), 16), ((1, 32, 64, 64), 4), ((2, 32, 64, 65), 4),
+          ((1, 100, 36, 37), 4), ((2, 40, 60, 61), 5)]
 
 
 def dev(t, g, nchw=True):
