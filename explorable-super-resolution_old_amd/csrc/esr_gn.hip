@@ -534,10 +534,11 @@ GnP params(int V, int64_t N, int64_t HW, int32_t C, int32_t G, const float *gamm
     p.gamma = gamma; p.beta = beta;
     p.N = (int)N; p.HW = HW; p.C = C; p.G = G; p.Cg = C / G; p.slope = slope;
     p.nb = (C + act8::BLK - 1) / act8::BLK;
-    // One workgroup per sample and chunk where that is at most 128 K values: 4 us for 3×40×36×64 against 17 us in three
-    // launches, break-even at twice the limit.
+    // One workgroup per sample and chunk where that is at most 64 K values: 46 K (3×40×36×64, chunks of 32 channels) take
+    // 15 us forward, as long as three launches, and two launches' host time (7 us) is saved; 96 K (16×31×31×100 in one
+    // chunk) take 29 us against 16 us in three.
     const int small = chunk_of(C, p.Cg), ln = (small + act8::BLK - 1) / act8::BLK * (act8::BLK / V);
-    const bool one = small <= SMALL_C && HW <= (128 << 10) / small;
+    const bool one = small <= SMALL_C && HW <= (64 << 10) / small;
     const int threads = one ? NTS : NT, lanes = one ? ln : p.nb * (act8::BLK / V);
     p.lanes = lanes < threads ? lanes : threads;
     p.step = one ? small : p.lanes * V;
