@@ -13,6 +13,9 @@ namespace act8 {
 
 constexpr int BLK = 32;
 
+// codes of a pixel: rows of 16 bytes, so that every pixel's codes start where a 16-byte access may
+__host__ __device__ __forceinline__ int pitch(int C) { return (C + 15) & ~15; }
+
 // exponent byte from the bits of max|x| (an unsigned max over abs bits orders finite < inf < NaN)
 __device__ __forceinline__ int exp_of(unsigned amax_bits) {
     const int q = (int)(amax_bits >> 23);

@@ -17,7 +17,7 @@ constexpr int NT = 256, UN = 4;
 
 struct Rows {
     long long P;
-    int C, nb, lanes, rpi;  // lanes: threads of a row (of this chunk); rpi: rows of a workgroup at a time
+    int C, nb, cp, lanes, rpi;  // cp: codes of a row; lanes: its threads (of this chunk); rpi: rows at a time
 };
 
 template <int V>
@@ -40,7 +40,7 @@ template <int V>
 __global__ __launch_bounds__(NT) void act8_pack_kernel(const float *x, Rows r, int8_t *codes, uint8_t *exps) {
     constexpr int L = act8::BLK / V;
     const int lane = threadIdx.x % r.lanes, ph = threadIdx.x / r.lanes, c = ((int)blockIdx.y * NT + lane) * V;
-    const bool in = c < r.C;
+    const bool in = c < r.C;  // (behind the last channel the code is 0)
     const long long p0 = (long long)blockIdx.x * r.rpi * UN + ph;
     if (ph >= r.rpi) return;
     float v[UN][V];
@@ -63,9 +63,9 @@ __global__ __launch_bounds__(NT) void act8_pack_kernel(const float *x, Rows r, i
         const long long p = p0 + (long long)j * r.rpi;
         int e;
         const uint32_t w = codes_of<V>(v[j], e);
-        if (!in || p >= r.P) continue;
-        if constexpr (V == 4) *reinterpret_cast<uint32_t *>(codes + p * r.C + c) = w;
-        else codes[p * r.C + c] = (int8_t)w;
+        if (c >= r.cp || p >= r.P) continue;
+        if constexpr (V == 4) *reinterpret_cast<uint32_t *>(codes + p * r.cp + c) = w;
+        else codes[p * r.cp + c] = (int8_t)w;
         if (lane % L == 0) exps[p * r.nb + c / act8::BLK] = (uint8_t)e;
     }
 }
@@ -80,8 +80,8 @@ __global__ __launch_bounds__(NT) void act8_unpack_kernel(const int8_t *codes, co
 #pragma unroll
     for (int j = 0; j < UN; ++j) {  // rows past the end read the last one and are not written
         const long long p = min(p0 + (long long)j * r.rpi, r.P - 1);
-        if constexpr (V == 4) w[j] = *reinterpret_cast<const uint32_t *>(codes + p * r.C + c);
-        else w[j] = (uint8_t)codes[p * r.C + c];
+        if constexpr (V == 4) w[j] = *reinterpret_cast<const uint32_t *>(codes + p * r.cp + c);
+        else w[j] = (uint8_t)codes[p * r.cp + c];
         e[j] = exps[p * r.nb + c / act8::BLK];
     }
 #pragma unroll
@@ -105,6 +105,7 @@ bool plan(int64_t P, int32_t C, int V, Rows &r, dim3 &grid) {
     r.P = flat ? P * (C / act8::BLK) : P;
     r.C = flat ? act8::BLK : C;
     r.nb = (r.C + act8::BLK - 1) / act8::BLK;
+    r.cp = act8::pitch(r.C);
     const int lanes = r.nb * (act8::BLK / V), chunks = (lanes + NT - 1) / NT;
     r.lanes = lanes < NT ? lanes : NT;
     r.rpi = NT / r.lanes;
@@ -114,15 +115,13 @@ bool plan(int64_t P, int32_t C, int V, Rows &r, dim3 &grid) {
     return true;
 }
 
-inline bool quads(const void *f32, const void *codes, int C) {
-    return C % 4 == 0 && (uintptr_t)f32 % 16 == 0 && (uintptr_t)codes % 4 == 0;
-}
+inline bool quads(const void *f32, int C) { return C % 4 == 0 && (uintptr_t)f32 % 16 == 0; }
 
 }  // namespace
 
 extern "C" int esr_act8_pack(const float *x, int64_t P, int32_t C, int8_t *codes, uint8_t *exps, esr_stream_t stream) {
-    if (!x || !codes || !exps || C <= 0) return ESR_EINVAL;
-    const int V = quads(x, codes, C) ? 4 : 1;
+    if (!x || !codes || !exps || C <= 0 || (uintptr_t)codes % 16) return ESR_EINVAL;
+    const int V = quads(x, C) ? 4 : 1;
     Rows r;
     dim3 grid;
     if (!plan(P, C, V, r, grid)) return ESR_EINVAL;
@@ -134,8 +133,8 @@ extern "C" int esr_act8_pack(const float *x, int64_t P, int32_t C, int8_t *codes
 
 extern "C" int esr_act8_unpack(const int8_t *codes, const uint8_t *exps, int64_t P, int32_t C, float *x,
                                esr_stream_t stream) {
-    if (!x || !codes || !exps || C <= 0) return ESR_EINVAL;
-    const int V = quads(x, codes, C) ? 4 : 1;
+    if (!x || !codes || !exps || C <= 0 || (uintptr_t)codes % 16) return ESR_EINVAL;
+    const int V = quads(x, C) ? 4 : 1;
     Rows r;
     dim3 grid;
     if (!plan(P, C, V, r, grid)) return ESR_EINVAL;

@@ -50,7 +50,7 @@ struct GnP {
     const double *grp;           // [N][G][8] per-group coefficients of the pass
     const double *sums, *sums_u; // [N][2][C]: s1, s2; [N][3][C]: Σu, Σu·x̂, Σu·gz
     long long HW;
-    int N, C, G, Cg, nb, lanes, rpi, step, chunks, splits, blocks;
+    int N, C, G, Cg, nb, cp, lanes, rpi, step, chunks, splits, blocks;
     float slope, eps;
 };
 
@@ -82,8 +82,8 @@ struct Raw {
     int e;
     __device__ __forceinline__ void load(const GnP &p, long long row, int c) {
         if constexpr (Q8) {
-            if constexpr (V == 4) w = *reinterpret_cast<const uint32_t *>(p.codes + row * p.C + c);
-            else w = (uint8_t)p.codes[row * p.C + c];
+            if constexpr (V == 4) w = *reinterpret_cast<const uint32_t *>(p.codes + row * p.cp + c);
+            else w = (uint8_t)p.codes[row * p.cp + c];
             e = p.exps[row * p.nb + c / act8::BLK];
         } else {
             load_f<V>(p.x, row * p.C + c, v);
@@ -298,19 +298,19 @@ __device__ __forceinline__ void put_blocks(const GnP &p, const float *v, bool ac
 #pragma unroll
     for (int k = 0; k < V; ++k) m = max(m, act8::abs_bits(v[k]));
     const int e = act8::exp_of(act8::block_max<L>(m));
-    if (!act) return;
+    if (c >= p.cp) return;  // (behind the last channel the code is 0)
     uint32_t w = 0;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
         float code = act8::code_of(v[k], e);
-        if (e != 255) {
+        if (act && e != 255) {
             const float at = act8::value_of(code, e);
             if (pre(at, k) != pre(v[k], k)) code += at > v[k] ? -1.f : 1.f;
         }
         w |= (uint32_t)(uint8_t)(int8_t)(int)code << (8 * k);
     }
-    if constexpr (V == 4) *reinterpret_cast<uint32_t *>(codes + row * p.C + c) = w;
-    else codes[row * p.C + c] = (int8_t)w;
+    if constexpr (V == 4) *reinterpret_cast<uint32_t *>(codes + row * p.cp + c) = w;
+    else codes[row * p.cp + c] = (int8_t)w;
     if (lane % L == 0) exps[row * p.nb + c / act8::BLK] = (uint8_t)e;
 }
 
@@ -512,13 +512,11 @@ inline bool shape_ok(int64_t N, int64_t HW, int32_t C, int32_t G) {
     return HW <= (1LL << 46) / C / N;  // element offsets, with room for the row arithmetic
 }
 inline bool bits_ok(const void *x, const void *codes, const void *exps) {
-    return x ? !codes && !exps : codes && exps;  // exactly one form of the input
+    return x ? !codes && !exps : codes && exps && (uintptr_t)codes % 16 == 0;  // exactly one form of the input
 }
-inline bool aligned(std::initializer_list<const void *> f32, std::initializer_list<const void *> codes) {
-    for (const void *q : f32)
+inline bool aligned(std::initializer_list<const void *> ptrs) {  // to 16 bytes
+    for (const void *q : ptrs)
         if ((uintptr_t)q % 16) return false;
-    for (const void *q : codes)
-        if ((uintptr_t)q % 4) return false;
     return true;
 }
 
@@ -534,6 +532,7 @@ GnP params(int V, int64_t N, int64_t HW, int32_t C, int32_t G, const float *gamm
     p.gamma = gamma; p.beta = beta;
     p.N = (int)N; p.HW = HW; p.C = C; p.G = G; p.Cg = C / G; p.slope = slope;
     p.nb = (C + act8::BLK - 1) / act8::BLK;
+    p.cp = act8::pitch(C);
     // One workgroup per sample and chunk where that is at most 64 K values: 46 K (3×40×36×64, chunks of 32 channels) take
     // 15 us forward, as long as three launches, and two launches' host time (7 us) is saved; 96 K (16×31×31×100 in one
     // chunk) take 29 us against 16 us in three.
@@ -605,10 +604,11 @@ extern "C" int64_t esr_gn_workspace_bytes(int64_t N, int64_t HW, int32_t C, int3
 extern "C" int esr_gn_lrelu_fwd(const float *x, int64_t N, int64_t HW, int32_t C, int32_t G, const float *gamma,
                                 const float *beta, float eps, float slope, float *y, double *stat, int8_t *codes,
                                 uint8_t *exps, int8_t *ycodes, uint8_t *yexps, void *ws, esr_stream_t stream) {
-    if (!x || !y || !stat || !ws || !shape_ok(N, HW, C, G) || !(eps >= 0.f) || !codes != !exps || !ycodes != !yexps)
+    if (!x || !y || !stat || !ws || !shape_ok(N, HW, C, G) || !(eps >= 0.f) || !codes != !exps || !ycodes != !yexps ||
+        !aligned({codes, ycodes}))
         return ESR_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
-    const int V = C % 4 == 0 && aligned({x, y}, {codes, ycodes}) ? 4 : 1;
+    const int V = C % 4 == 0 && aligned({x, y}) ? 4 : 1;
     GnP p = params(V, N, HW, C, G, gamma, beta, slope);
     p.x = x; p.eps = eps;
     pass<0>(p, V, codes || ycodes, GnOut{y, nullptr, nullptr, nullptr, codes, ycodes, exps, yexps}, (double *)ws, nullptr,
@@ -622,7 +622,7 @@ extern "C" int esr_gn_lrelu_bwd(const float *x, const int8_t *codes, const uint8
                                 void *ws, esr_stream_t stream) {
     if (!bits_ok(x, codes, exps) || !gy || !gx || !stat || !sums_ || !ws || !shape_ok(N, HW, C, G)) return ESR_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
-    const int V = C % 4 == 0 && aligned({x, gy, gx}, {codes}) ? 4 : 1;
+    const int V = C % 4 == 0 && aligned({x, gy, gx}) ? 4 : 1;
     GnP p = params(V, N, HW, C, G, gamma, beta, slope);
     p.x = x; p.codes = codes; p.exps = exps; p.gy = gy; p.stat = stat;
     double *partial = (double *)ws, *grp = partial + N * p.splits * 3 * C + N * 3 * C;
@@ -638,7 +638,7 @@ extern "C" int esr_gn_lrelu_bwd2(const float *x, const int8_t *codes, const uint
     if (!bits_ok(x, codes, exps) || !gy || !stat || !sums_ || !g_x || !g_gy || !ws || !shape_ok(N, HW, C, G))
         return ESR_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
-    const int V = C % 4 == 0 && aligned({x, gy, u, g_x, g_gy}, {codes}) ? 4 : 1;
+    const int V = C % 4 == 0 && aligned({x, gy, u, g_x, g_gy}) ? 4 : 1;
     GnP p = params(V, N, HW, C, G, gamma, beta, slope);
     p.x = x; p.codes = codes; p.exps = exps; p.gy = gy; p.u = u; p.gga = gg_gamma; p.ggb = gg_beta; p.stat = stat;
     p.sums = sums_;

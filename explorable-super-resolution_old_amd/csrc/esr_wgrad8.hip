@@ -37,7 +37,7 @@ struct WgP {
     const int8_t *codes;
     const uint8_t *exps;
     const float *dy;
-    int B, Hs, Ws, cin, nb, MH, MW, cout, k, s, p, nci, nco, groups;
+    int B, Hs, Ws, cin, cp, nb, MH, MW, cout, k, s, p, nci, nco, groups;
     int tY, tX, tiles, per_split, splits;  // K steps: rows and columns of tiles per image, all, per split
     float *partial;                        // [splits][k·k][nci·64][nco·64]
 };
@@ -66,9 +66,8 @@ struct Shape {
     static constexpr int NX = (ROWS * COLS * 4 + NT - 1) / NT, NG = KPX * 16 / NT;
 };
 
-// LV: how channels are loaded. 0: 16 codes and 4 gradients at once (cin a multiple of 16, cout of 4); 1: by fours; 2: one
-// by one.
-template <int KR, int KC, int S, int TG, int LV>
+// G4: four gradients at once (cout a multiple of 4), or one by one.
+template <int KR, int KC, int S, int TG, bool G4>
 __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
     using H = Shape<KR, KC, S, TG>;
     constexpr int RY = H::RY;
@@ -99,7 +98,7 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
     }
     // Every load is issued, from the tensor's first element where its place is outside, and its value dropped when it is
     // expanded: no branch for which the loads in flight would have to be waited for.
-    uint32_t rx[H::NX][4];
+    uint4 rx[H::NX];
     int re[H::NX], ok = 0;
     f32x4 rg[H::NG];
     auto load = [&](int t) {
@@ -107,7 +106,7 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
         const int Y0 = ty * RY, X0 = (r - ty * p.tX) * 16;
         const int st = H::ONE ? p.s : 1, ys = Y0 * (H::ONE ? p.s : S) + oy, xs = X0 * (H::ONE ? p.s : S) + ox;
         const long long pix0 = (long long)img * p.Hs * p.Ws;
-        const int8_t *codes = p.codes + pix0 * p.cin;
+        const int8_t *codes = p.codes + pix0 * p.cp;
         const uint8_t *exps = p.exps + pix0 * p.nb;
         const float *dy = p.dy + (long long)img * p.MH * p.MW * p.cout;
         ok = 0;
@@ -118,24 +117,7 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
             const unsigned m = -(unsigned)in, pix = (unsigned)(sy * p.Ws + sx) & m, c = (unsigned)ci & m;  // (no branch)
             ok |= (int)in << j;
             re[j] = exps[pix * (unsigned)p.nb + c / act8::BLK];
-            const int8_t *src = codes + (pix * (unsigned)p.cin + c);
-            if constexpr (LV == 0) {
-                const uint4 q = *reinterpret_cast<const uint4 *>(src);
-                rx[j][0] = q.x; rx[j][1] = q.y; rx[j][2] = q.z; rx[j][3] = q.w;
-            } else {
-                const int n = in ? p.cin - ci : 1;  // channels there are (>= 1)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (LV == 1) {
-                        rx[j][i] = *reinterpret_cast<const uint32_t *>(src + (4 * i < n ? 4 * i : 0));
-                    } else {
-                        rx[j][i] = 0;
-#pragma unroll
-                        for (int b = 0; b < 4; ++b)
-                            rx[j][i] |= (uint32_t)(uint8_t)src[4 * i + b < n ? 4 * i + b : 0] << (8 * b);
-                    }
-                }
-            }
+            rx[j] = *reinterpret_cast<const uint4 *>(codes + (pix * (unsigned)p.cp + c));
         }
 #pragma unroll
         for (int j = 0; j < H::NG; ++j) {
@@ -143,7 +125,7 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
             const bool in = Y < p.MH && X < p.MW && co < p.cout;
             const float *src = dy + (((unsigned)(Y * p.MW + X) * (unsigned)p.cout + co) & -(unsigned)in);
             ok |= (int)in << (16 + j);
-            if constexpr (LV < 2) {
+            if constexpr (G4) {
                 rg[j] = *reinterpret_cast<const f32x4 *>(src);
             } else {
                 const int n = in ? p.cout - co : 1;
@@ -155,20 +137,15 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
     auto drop = [&]() {  // the values that are outside
 #pragma unroll
         for (int j = 0; j < H::NX; ++j) {
-            const bool in = ok >> j & 1;
-            const int n = p.cin - ci0 - 16 * (tid & 3);
-            re[j] = in ? re[j] : 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (LV == 2) rx[j][i] &= n >= 4 * i + 4 ? ~0u : n <= 4 * i ? 0u : (1u << (8 * (n - 4 * i))) - 1;
-                rx[j][i] = in && (LV != 1 || 4 * i < n) ? rx[j][i] : 0;
-            }
+            const unsigned m = -(unsigned)(ok >> j & 1);
+            re[j] &= m;
+            rx[j] = make_uint4(rx[j].x & m, rx[j].y & m, rx[j].z & m, rx[j].w & m);
         }
 #pragma unroll
         for (int j = 0; j < H::NG; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                rg[j][i] = (ok >> (16 + j) & 1) && (LV < 2 || co0 + 4 * (tid & 15) + i < p.cout) ? rg[j][i] : 0.f;
+                rg[j][i] = (ok >> (16 + j) & 1) && (G4 || co0 + 4 * (tid & 15) + i < p.cout) ? rg[j][i] : 0.f;
     };
 
     f32x16 acc[KR * KC];
@@ -221,10 +198,11 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
             me = max(me, re[j] == 255 ? 0 : re[j]);
             const _Float16 sc = re[j] == 255 ? (_Float16)__builtin_nanf("") : (_Float16)ldexpf(1.f, min(re[j] - ex, 2) + 3);
             const f16x2 s = {sc, sc}, off = s * (_Float16)-1152.f;
+            const uint32_t q[4] = {rx[j].x, rx[j].y, rx[j].z, rx[j].w};
             f16x2 o[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t u = rx[j][i] ^ 0x80808080u;
+                const uint32_t u = q[i] ^ 0x80808080u;
                 o[2 * i] = code_pair(u, 0x04010400u, s, off);
                 o[2 * i + 1] = code_pair(u, 0x04030402u, s, off);
             }
@@ -357,11 +335,11 @@ bool geometry(int64_t B, int32_t Hs, int32_t Ws, int32_t cin, int32_t MH, int32_
     if (Hs + 2 * pad < k || Ws + 2 * pad < k) return false;
     if (MH != (Hs + 2 * pad - k) / s + 1 || MW != (Ws + 2 * pad - k) / s + 1) return false;
     // (offsets within an image are 32-bit)
-    if ((int64_t)MH * MW > 0x7fffffffLL / cout / 4 || (int64_t)Hs * Ws > 0x7fffffffLL / cin || B > 0x7fffffff) return false;
+    if ((int64_t)MH * MW > 0x7fffffffLL / cout / 4 || (int64_t)Hs * Ws > 0x7fffffffLL / act8::pitch(cin) || B > 0x7fffffff) return false;
     g.kind = k == 3 && s == 1 ? 0 : k == 4 && s == 2 ? 1 : k == 4 && s == 1 ? 2 : k == 8 && s == 1 ? 3 : 4;
     WgP &p = g.p;
     p = WgP{};
-    p.B = (int)B; p.Hs = Hs; p.Ws = Ws; p.cin = cin; p.nb = (cin + 31) / 32; p.MH = MH; p.MW = MW; p.cout = cout;
+    p.B = (int)B; p.Hs = Hs; p.Ws = Ws; p.cin = cin; p.cp = act8::pitch(cin); p.nb = (cin + 31) / 32; p.MH = MH; p.MW = MW; p.cout = cout;
     p.k = k; p.s = s; p.p = pad;
     p.nci = (cin + 63) / 64;
     p.nco = (cout + 63) / 64;
@@ -371,23 +349,34 @@ bool geometry(int64_t B, int32_t Hs, int32_t Ws, int32_t cin, int32_t MH, int32_
     const long long tiles = B * p.tY * p.tX, work = (long long)p.nci * p.nco * p.groups;
     if (tiles > 0x7fffffffLL || work > (1 << 24)) return false;
     p.tiles = (int)tiles;
-    // a workgroup for every place (two per CU, one of the eight-wave kind), a K step each at least
-    const long long places = g.kind == 1 ? 256 : 512, n = work >= places ? 1 : places / work;
-    p.per_split = (int)((tiles + (n < tiles ? n : tiles) - 1) / (n < tiles ? n : tiles));
+    // Splits: a K step takes about 1 + 0.19·taps us with a workgroup on each CU and 1.45 of that with two (3×3, measured:
+    // 2.7 and 3.9 us), and a split's partial sums are written and read again at some 5 TB/s.  The cheapest of the numbers
+    // that fill the CUs once or twice, or a half, a quarter ... of them.
+    const long long places = g.kind == 1 ? 256 : 512;
+    const double step = 1.0 + 0.19 * k * k / p.groups, mb = 4e-6 * k * k * 4096.0 * p.nci * p.nco;
+    double best = 0;
+    for (long long n = work >= places ? 1 : places / work; n; n /= 2) {
+        const long long per = (tiles + n - 1) / n, used = (tiles + per - 1) / per;
+        const double cost = per * step * (work * used > 256 ? 1.45 : 1.0) + 0.4 * mb * used;
+        if (best == 0 || cost < best) {
+            best = cost;
+            p.per_split = (int)per;
+        }
+    }
     p.splits = (p.tiles + p.per_split - 1) / p.per_split;
     return (long long)(p.splits + 7) / 8 * 8 * work <= 0x7fffffffLL;
 }
 
-template <int LV>
+template <bool G4>
 void run(const Geo &g, hipStream_t st) {
     const WgP &p = g.p;
     const dim3 grid((unsigned)((p.splits + 7) / 8 * 8 * p.nci * p.nco * p.groups)), block(NT);
     switch (g.kind) {
-        case 0: hipLaunchKernelGGL((wgrad8_kernel<3, 3, 1, 1, LV>), grid, block, 0, st, p); break;
-        case 1: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 2, 2, LV>), grid, dim3(2 * NT), 0, st, p); break;
-        case 2: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 1, 1, LV>), grid, block, 0, st, p); break;
-        case 3: hipLaunchKernelGGL((wgrad8_kernel<1, 8, 1, 1, LV>), grid, block, 0, st, p); break;
-        default: hipLaunchKernelGGL((wgrad8_kernel<1, 1, 1, 1, LV>), grid, block, 0, st, p);
+        case 0: hipLaunchKernelGGL((wgrad8_kernel<3, 3, 1, 1, G4>), grid, block, 0, st, p); break;
+        case 1: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 2, 2, G4>), grid, dim3(2 * NT), 0, st, p); break;
+        case 2: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 1, 1, G4>), grid, block, 0, st, p); break;
+        case 3: hipLaunchKernelGGL((wgrad8_kernel<1, 8, 1, 1, G4>), grid, block, 0, st, p); break;
+        default: hipLaunchKernelGGL((wgrad8_kernel<1, 1, 1, 1, G4>), grid, block, 0, st, p);
     }
 }
 
@@ -404,15 +393,12 @@ extern "C" int esr_dconv_wgrad_act8(const int8_t *codes, const uint8_t *exps, in
                                     int32_t cin, const float *dy, int32_t MH, int32_t MW, int32_t cout, int32_t k,
                                     int32_t s, int32_t pad, float *gw, void *ws, esr_stream_t stream) {
     Geo g;
-    if (!codes || !exps || !dy || !gw || !ws || !geometry(B, Hs, Ws, cin, MH, MW, cout, k, s, pad, g)) return ESR_EINVAL;
+    if (!codes || !exps || !dy || !gw || !ws || (uintptr_t)codes % 16 || (uintptr_t)ws % 16 || !geometry(B, Hs, Ws, cin, MH, MW, cout, k, s, pad, g)) return ESR_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
     WgP &p = g.p;
     p.codes = codes; p.exps = exps; p.dy = dy; p.partial = (float *)ws;
-    const bool v16 = cin % 16 == 0 && (uintptr_t)codes % 16 == 0, g4 = cout % 4 == 0 && (uintptr_t)dy % 16 == 0;
-    const int lv = v16 && g4 ? 0 : cin % 4 == 0 && (uintptr_t)codes % 4 == 0 && g4 ? 1 : 2;
-    if (lv == 0) run<0>(g, st);
-    else if (lv == 1) run<1>(g, st);
-    else run<2>(g, st);
+    if (cout % 4 == 0 && (uintptr_t)dy % 16 == 0) run<true>(g, st);
+    else run<false>(g, st);
     hipLaunchKernelGGL(wgrad8_reduce, dim3((unsigned)((cout + 31) / 32) * cin * k * k), dim3(NT), 0, st, p.partial, p.splits,
                        k * k, cin, cout, p.nci * 64, p.nco * 64, gw);
     return hipGetLastError() == hipSuccess ? ESR_OK : ESR_ELAUNCH;

@@ -49,29 +49,35 @@ def check_dev(what, *ts):
     return dev
 
 
+def pitch(C):
+    """Codes of a pixel of C channels: rows of 16 bytes."""
+    return -(-C // 16) * 16
+
+
 def empty_blocks(shape, dev):
     """Unwritten (codes, exps) of an activation of `shape` [..., C]."""
-    return (torch.empty(shape, device=dev, dtype=torch.int8),
-            torch.empty(tuple(shape[:-1]) + (-(-shape[-1] // BLOCK),), device=dev, dtype=torch.uint8))
+    lead, C = tuple(shape[:-1]), shape[-1]
+    return (torch.empty(lead + (pitch(C),), device=dev, dtype=torch.int8),
+            torch.empty(lead + (-(-C // BLOCK),), device=dev, dtype=torch.uint8))
 
 
 class Act8:
-    """An activation [..., C] in 8 bits: codes int8 [..., C], exps uint8 [..., ceil(C / 32)]; the value of a code is
-    code · 2^(e − 132), NaN where e = 255."""
-    __slots__ = ('codes', 'exps')
+    """An activation of `shape` [..., C] in 8 bits: codes int8 [..., C rounded up to 16] and exps uint8
+    [..., ceil(C / 32)]; the value of a code is code · 2^(e − 132), NaN where e = 255."""
+    __slots__ = ('codes', 'exps', 'shape')
 
-    def __init__(self, codes, exps):
-        if codes.dtype != torch.int8 or exps.dtype != torch.uint8 or codes.dim() < 1 or \
-                tuple(exps.shape) != tuple(codes.shape[:-1]) + (-(-codes.shape[-1] // BLOCK),):
-            raise ValueError('Act8: int8 codes [..., C] with uint8 exponents [..., ceil(C / 32)], got %s %s and %s %s'
-                             % (codes.dtype, tuple(codes.shape), exps.dtype, tuple(exps.shape)))
+    def __init__(self, codes, exps, channels):
+        lead = tuple(codes.shape[:-1])
+        if codes.dtype != torch.int8 or exps.dtype != torch.uint8 or codes.dim() < 1 or channels < 1 or \
+                codes.shape[-1] != pitch(channels) or tuple(exps.shape) != lead + (-(-channels // BLOCK),):
+            raise ValueError('Act8: int8 codes [..., %d] with uint8 exponents [..., %d] for %d channels, got %s %s and %s %s'
+                             % (pitch(channels), -(-channels // BLOCK), channels, codes.dtype, tuple(codes.shape),
+                                exps.dtype, tuple(exps.shape)))
         if codes.device != exps.device:
             raise RuntimeError('Act8: codes on %s, exponents on %s' % (codes.device, exps.device))
-        self.codes, self.exps = codes.contiguous(), exps.contiguous()
-
-    @property
-    def shape(self):
-        return self.codes.shape
+        codes = codes.contiguous()
+        self.codes = codes if codes.data_ptr() % 16 == 0 else codes.clone()
+        self.exps, self.shape = exps.contiguous(), lead + (channels,)
 
     @property
     def nbytes(self):
@@ -94,15 +100,15 @@ def pack(x):
     """Act8 of a float32 tensor [..., C] (channels last; a copy is made of one that is not contiguous).  Not
     differentiable: what the backward keeps, not an operation of the forward."""
     check_dev('act8', x)
-    if x.dim() < 1:
-        raise ValueError('act8.pack: a tensor [..., C], got a scalar')
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError('act8.pack: a tensor [..., C], got %s' % (tuple(x.shape),))
     x = x.detach().contiguous()
     codes, exps = empty_blocks(x.shape, x.device)
     if x.numel():
         with on(x.device):
             _lib.check(_lib.load().esr_act8_pack(x.data_ptr(), x.numel() // x.shape[-1], x.shape[-1], codes.data_ptr(),
                                                  exps.data_ptr(), stream(x.device)), 'esr_act8_pack')
-    return Act8(codes, exps)
+    return Act8(codes, exps, x.shape[-1])
 
 
 class Carrier(torch.autograd.Function):

@@ -410,7 +410,7 @@ class WgradAct8Fn(torch.autograd.Function):
     def forward(ctx, carrier, gy, codes, exps, k, s, p, prec=None):
         ctx.save_for_backward(carrier, gy, codes, exps)
         ctx.geom = (k, s, p, prec)
-        return conv_wgrad_act8(act8.Act8(codes, exps), gy, k, s, p)
+        return conv_wgrad_act8(act8.Act8(codes, exps, carrier.shape[3]), gy, k, s, p)
 
     @staticmethod
     def backward(ctx, ggw):
@@ -419,7 +419,7 @@ class WgradAct8Fn(torch.autograd.Function):
         ggw = ggw.contiguous()
         g_x = DgradFn.apply(gy, ggw, k, s, p, carrier.shape[1], carrier.shape[2], prec) \
             if ctx.needs_input_grad[0] else None
-        g_gy = DConvFn.apply(act8.Act8(codes, exps).unpack(), ggw, None, k, s, p, prec) \
+        g_gy = DConvFn.apply(act8.Act8(codes, exps, carrier.shape[3]).unpack(), ggw, None, k, s, p, prec) \
             if ctx.needs_input_grad[1] else None
         return g_x, g_gy, None, None, None, None, None, None
 
@@ -527,7 +527,7 @@ def _df_bwd(xh, gy, mask, slope, w, need_x, need_w):
 
 def _df_mask(y, y8):
     """The layer's output, or its 8-bit values (their y > 0 is the output's) where it was kept so."""
-    return y if y8 is None else act8.Act8(*y8).unpack()
+    return y if y8 is None else act8.Act8(*y8, 64).unpack()
 
 
 class _DFirstFn(torch.autograd.Function):
@@ -628,7 +628,7 @@ def dfirst_lrelu8(x, conv, slope):
         xh = _ToNHWC.apply(x)
     if conv.keeps8():
         y, *y8 = _DFirstFn.apply(xh, conv.weight, conv.bias, float(slope), True)
-        return y.permute(0, 3, 1, 2), act8.Act8(*y8)
+        return y.permute(0, 3, 1, 2), act8.Act8(*y8, 64)
     return _DFirstFn.apply(xh, conv.weight, conv.bias, float(slope)).permute(0, 3, 1, 2), None
 
 

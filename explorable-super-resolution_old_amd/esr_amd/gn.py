@@ -151,13 +151,13 @@ def group_norm_lrelu(x, groups, weight=None, bias=None, eps=1e-5, slope=0.2, che
     dev = act8.check_dev('gn', x, weight, bias)
     if B == 0:
         y = x * 1.0
-        return (y, act8.Act8(*act8.empty_blocks((0, H, W, C), dev))) if out8 else y
+        return (y, act8.Act8(*act8.empty_blocks((0, H, W, C), dev), C)) if out8 else y
     x = _nhwc(x)
     weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
     needs = checkpoint and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))
     out = _GNLReLUFn.apply(x, act8.Carrier.apply(x) if needs else None, weight, bias, int(groups), float(eps),
                            float(slope), bool(out8))
-    return (out[0], act8.Act8(*out[1:])) if out8 else out
+    return (out[0], act8.Act8(*out[1:], C)) if out8 else out
 
 
 class HipGroupNorm(nn.GroupNorm):

@@ -462,14 +462,16 @@ int esr_bn_lrelu_bwd2(const float *x, const float *gy, const float *u, const flo
 
 /* ---- activations kept in 8 bits (esr_act8.hip, esr_wgrad8.hip) ------------------------------------------------------
  * What the discriminator's blocks keep of an activation x [P][C] (P pixels, channels last) from the forward to the
- * backward pass: codes int8 [P][C] and one exponent byte per 32 channels of a pixel, exps [P][ceil(C / 32)]; the value
+ * backward pass: codes int8 [P][16 * ceil(C / 16)] (16-byte aligned; 0 behind channel C), and one exponent byte per 32
+ * channels of a pixel, exps [P][ceil(C / 32)]; the value
  * of a code is code · 2^(e − 132), e the smallest with 127 · 2^(e − 132) >= the block's max |x| (e = 255: the block
  * holds an infinity or a NaN and reads back as NaN).  Error <= half a step <= max|x|/127; x > 0 is kept exactly (a
  * positive value never takes code 0).  C need not be a multiple of 32 or of 4.
  * esr_dconv_wgrad_act8: the weight gradient of conv2d(x, w, stride s, zero padding pad) from x's blocks:
  *   gw[co][ci][ky][kx] = sum over b, Y, X of x[b, s*Y + ky - pad, s*X + kx - pad, ci] * dy[b, Y, X, co]
  * x [B][Hs][Ws][cin], dy [B][MH][MW][cout] fp32, MH = (Hs + 2·pad − k) / s + 1 (likewise MW), k <= 8, gw in torch's
- * layout; ws = esr_dconv_wgrad_act8_workspace_bytes(...) bytes (ESR_EINVAL on bad arguments).  Deterministic. */
+ * layout; ws = esr_dconv_wgrad_act8_workspace_bytes(...) bytes, 16-byte aligned (ESR_EINVAL on bad arguments).
+ * Deterministic. */
 int esr_act8_pack(const float *x, int64_t P, int32_t C, int8_t *codes, uint8_t *exps, esr_stream_t stream);
 int esr_act8_unpack(const int8_t *codes, const uint8_t *exps, int64_t P, int32_t C, float *x, esr_stream_t stream);
 int64_t esr_dconv_wgrad_act8_workspace_bytes(int64_t B, int32_t Hs, int32_t Ws, int32_t cin, int32_t MH, int32_t MW,

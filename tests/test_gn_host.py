@@ -75,16 +75,16 @@ def test_refusals():
         with pytest.raises(ValueError):
             bad()
     for bad in (lambda: gn.group_norm_lrelu(x, 2), lambda: gn.HipGroupNorm(2, 8)(x), lambda: act8.pack(x),
-                lambda: act8.Act8(torch.zeros(2, 40, dtype=torch.int8), torch.zeros(2, 2, dtype=torch.uint8)).unpack()):
+                lambda: act8.Act8(torch.zeros(2, 48, dtype=torch.int8), torch.zeros(2, 2, dtype=torch.uint8), 40).unpack()):
         with pytest.raises(RuntimeError, match='ROCm device'):
             bad()
-    with pytest.raises(ValueError):
-        act8.Act8(torch.zeros(2, 40, dtype=torch.int8), torch.zeros(2, 1, dtype=torch.uint8))
-    with pytest.raises(ValueError):
-        act8.Act8(torch.zeros(2, 40), torch.zeros(2, 2, dtype=torch.uint8))
+    i8, u8 = (lambda *s: torch.zeros(*s, dtype=torch.int8)), (lambda *s: torch.zeros(*s, dtype=torch.uint8))
+    for bad in ((i8(2, 48), u8(2, 1), 40), (torch.zeros(2, 48), u8(2, 2), 40), (i8(2, 40), u8(2, 2), 40),
+                (i8(2, 48), i8(2, 2), 40), (i8(2, 48), u8(2, 2), 49), (i8(2, 0), u8(2, 0), 0)):
+        with pytest.raises(ValueError):
+            act8.Act8(*bad)
     with pytest.raises(RuntimeError, match='ROCm device'):
-        dconv.conv_wgrad_act8(act8.Act8(torch.zeros(1, 4, 4, 8, dtype=torch.int8),
-                                        torch.zeros(1, 4, 4, 1, dtype=torch.uint8)), torch.zeros(1, 4, 4, 8), 3, 1, 1)
+        dconv.conv_wgrad_act8(act8.Act8(i8(1, 4, 4, 16), u8(1, 4, 4, 1), 8), torch.zeros(1, 4, 4, 8), 3, 1, 1)
     conv = dconv.HipConv2d(8, 8, 3, padding=1)
     conv.act_checkpoint = 'int4'
     with pytest.raises(ValueError):
@@ -99,6 +99,7 @@ def test_c_entries_refuse():
     assert lib.esr_act8_pack(None, 1, 1, p, p, None) == E and lib.esr_act8_pack(p, 0, 4, p, p, None) == E
     assert lib.esr_act8_unpack(p, None, 1, 1, p, None) == E and lib.esr_act8_unpack(p, p, 1, 0, p, None) == E
     assert lib.esr_act8_pack(p, 1 << 45, 64, p, p, None) == E
+    assert lib.esr_act8_pack(p, 1, 1, p + 4, p, None) == E and lib.esr_act8_unpack(p + 8, p, 1, 1, p, None) == E  # alignment
     ok = (2, 16, 8, 4)
     assert lib.esr_gn_workspace_bytes(*ok) > 0
     for bad in ((0, 16, 8, 4), (2, 0, 8, 4), (2, 16, 8, 3), (2, 16, 0, 1), (2, 16, 8, 0), (70000, 16, 8, 4),
@@ -110,7 +111,7 @@ def test_c_entries_refuse():
         assert lib.esr_gn_lrelu_fwd(p, *ok, None, None, 1e-5, 0.2, p, p, *blocks, p, None) == E
     assert lib.esr_gn_lrelu_bwd(p, None, None, p, *ok, None, None, p, 0.2, None, p, p, p, p, None) == E
     bwd = lambda x, c, e: lib.esr_gn_lrelu_bwd(x, c, e, p, *ok, None, None, p, 0.2, p, p, p, p, p, None)  # noqa: E731
-    assert bwd(None, None, None) == E and bwd(p, p, p) == E and bwd(None, p, None) == E
+    assert bwd(None, p + 4, p) == E and bwd(None, None, None) == E and bwd(p, p, p) == E and bwd(None, p, None) == E
     assert lib.esr_gn_lrelu_bwd2(None, p, p, p, None, None, None, *ok, None, None, p, 0.2, None, p, p, p, p, None) == E
     geo = (2, 8, 8, 64, 8, 8, 64, 3, 1, 1)
     n = lib.esr_dconv_wgrad_act8_workspace_bytes(*geo)
@@ -121,6 +122,7 @@ def test_c_entries_refuse():
         assert lib.esr_dconv_wgrad_act8_workspace_bytes(*bad) == E, (i, v)
         assert lib.esr_dconv_wgrad_act8(p, p, *bad[:4], p, *bad[4:], p, p, None) == E, (i, v)
     assert lib.esr_dconv_wgrad_act8(p, None, *geo[:4], p, *geo[4:], p, p, None) == E
+    assert lib.esr_dconv_wgrad_act8(p + 4, p, *geo[:4], p, *geo[4:], p, p, None) == E
 
 
 def _opt(**d):

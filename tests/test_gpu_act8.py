@@ -23,9 +23,10 @@ def test_pack_is_the_definition(gpu_device, P, C):
     x = (rng.standard_normal((P, C)) * np.exp2(rng.integers(-20, 20, (P, 1)))).astype(np.float32)
     codes, exps, v = R.pack(x)
     q = act8.pack(torch.from_numpy(x).to(gpu_device))
-    assert np.array_equal(q.codes.cpu().numpy(), codes) and np.array_equal(q.exps.cpu().numpy(), exps)
+    got = q.codes.cpu().numpy()
+    assert np.array_equal(got[:, :C], codes) and not got[:, C:].any() and np.array_equal(q.exps.cpu().numpy(), exps)
     assert np.array_equal(q.unpack().cpu().numpy(), v.astype(np.float32))
-    assert q.nbytes == P * (C + -(-C // 32))
+    assert q.nbytes == P * (-(-C // 16) * 16 + -(-C // 32)) and q.shape == (P, C)
 
 
 def test_pack_extremes(gpu_device):
@@ -62,8 +63,8 @@ def test_pack_layouts(gpu_device):
         q = act8.pack(v)
         assert torch.equal(q.codes, want.codes) and torch.equal(q.exps, want.exps)
     assert act8.pack(x[:0]).unpack().shape == (0, 5, 7, 40)
-    codes = torch.empty(x.numel() + 1, device=gpu_device, dtype=torch.int8)[1:].view(x.shape).copy_(want.codes)
-    assert torch.equal(act8.Act8(codes, want.exps).unpack(), want.unpack())
+    codes = torch.empty(want.codes.numel() + 1, device=gpu_device, dtype=torch.int8)[1:].view(want.codes.shape)
+    assert torch.equal(act8.Act8(codes.copy_(want.codes), want.exps, 40).unpack(), want.unpack())
 
 
 # B, H, W, Ci, Co, k, s, p: every layer kind of the discriminator, ragged channels, maps smaller than the kernel's reach,
