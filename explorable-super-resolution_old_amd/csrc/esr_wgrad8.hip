@@ -323,6 +323,29 @@ __global__ __launch_bounds__(NT) void wgrad8_reduce(const float *partial, int sp
     }
 }
 
+// The same for many weights (and so few splits): a workgroup adds 32 co × cb ci × all taps (at most 64 of the latter two) and
+// writes them by rows of one co, which lie together in gw (one by one, at a stride of cin·T, each would cost a sector).
+__global__ __launch_bounds__(NT) void wgrad8_reduce_rows(const float *partial, int splits, int T, int cin, int cout, int cip,
+                                                         int cop, int cb, float *gw) {
+    __shared__ float tile[32][65];
+    const int nco = (cout + 31) / 32, co0 = blockIdx.x % nco * 32, ci0 = blockIdx.x / nco * cb, n = min(cb, cin - ci0) * T;
+    const long long step = (long long)T * cip * cop;
+    for (int i = threadIdx.x; i < n * 8; i += NT) {
+        const int o = 4 * (i & 7), r = i >> 3, ci = ci0 + r / T, t = r % T;
+        const float *src = partial + ((long long)t * cip + ci) * cop + co0 + o;
+        f32x4 v = *reinterpret_cast<const f32x4 *>(src);
+#pragma unroll 4
+        for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4 *>(src + s * step);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tile[o + k][r] = v[k];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * n; i += NT) {
+        const int o = i / n, r = i - o * n;
+        if (co0 + o < cout) gw[((long long)(co0 + o) * cin + ci0) * T + r] = tile[o][r];
+    }
+}
+
 struct Geo {
     int kind;  // 0: 3×3, 1: 4×4 stride 2, 2: 4×4 stride 1, 3: 8×8, 4: tap by tap
     WgP p;
@@ -399,7 +422,13 @@ extern "C" int esr_dconv_wgrad_act8(const int8_t *codes, const uint8_t *exps, in
     p.codes = codes; p.exps = exps; p.dy = dy; p.partial = (float *)ws;
     if (cout % 4 == 0 && (uintptr_t)dy % 16 == 0) run<true>(g, st);
     else run<false>(g, st);
-    hipLaunchKernelGGL(wgrad8_reduce, dim3((unsigned)((cout + 31) / 32) * cin * k * k), dim3(NT), 0, st, p.partial, p.splits,
-                       k * k, cin, cout, p.nci * 64, p.nco * 64, gw);
+    const int T = k * k, nco = (cout + 31) / 32, cb = T < 64 ? 64 / T : 1;
+    const long long rows = (long long)nco * ((cin + cb - 1) / cb);
+    if (rows >= 256)  // enough workgroups without cutting the splits (64->512 8x8 of 8 images: 75 -> 43 us in all)
+        hipLaunchKernelGGL(wgrad8_reduce_rows, dim3((unsigned)rows), dim3(NT), 0, st, p.partial, p.splits, T, cin, cout,
+                           p.nci * 64, p.nco * 64, cb, gw);
+    else
+        hipLaunchKernelGGL(wgrad8_reduce, dim3((unsigned)nco * cin * T), dim3(NT), 0, st, p.partial, p.splits, T, cin, cout,
+                           p.nci * 64, p.nco * 64, gw);
     return hipGetLastError() == hipSuccess ? ESR_OK : ESR_ELAUNCH;
 }
