@@ -103,7 +103,8 @@ def pack(x, pre=None):
     wide = lambda t: np.repeat(t, 32, 1)[:, :C]  # noqa: E731
     step, fine = wide(np.ldexp(1.0, k)), wide(ok)
     xs = np.where(fine, x, 0)
-    code = np.rint(xs / step)
+    most = np.where(wide(k) == 122, 63, 127)  # 64 · 2^122 is past the largest float
+    code = np.clip(np.rint(xs / step), -most, most)
     pre = pre or (lambda v: v)
     wrong = fine & ((pre(code * step) > 0) != (pre(xs) > 0))
     code = code + np.where(wrong, np.where(code * step > xs, -1.0, 1.0), 0.0)

@@ -49,8 +49,8 @@ def test_pack_extremes(gpu_device):
     codes, exps, v = R.pack(x)
     q = act8.pack(torch.from_numpy(x).to(gpu_device))
     assert np.array_equal(q.exps.cpu().numpy(), exps) and np.array_equal(q.codes.cpu().numpy(), codes)
-    with np.errstate(over='ignore'):  # 127 steps of the largest float's block round to infinity in the reference too
-        np.testing.assert_array_equal(q.unpack().cpu().numpy(), v.astype(f))
+    np.testing.assert_array_equal(q.unpack().cpu().numpy(), v.astype(f))
+    assert np.isfinite(v[1]).all()
 
 
 def test_pack_layouts(gpu_device):
@@ -212,6 +212,68 @@ def test_conv_layer_checkpoint(gpu_device, k, s, p):
         convs[1](x, act8.pack(torch.zeros(1, 2, 2, 64, device=gpu_device)))
 
 
+def test_conv_layer_graph_capture(gpu_device):
+    """A checkpointed layer's forward, backward and double backward captured once, replayed between eager calls."""
+    m = dconv.HipConv2d(64, 32, 3, padding=1).to(gpu_device)
+    m.act_checkpoint = 'int8'
+    w0, b0 = m.weight.detach(), m.bias.detach()
+    shape = (2, 64, 12, 14)
+    mk = lambda c: torch.randn(2, c, 12, 14, device=gpu_device).contiguous(  # noqa: E731
+        memory_format=torch.channels_last)
+    static = [mk(64), mk(32), mk(64)]
+
+    def step(x, gy, u):
+        x, gy = x.detach().requires_grad_(), gy.detach().requires_grad_()
+        w, b = w0.detach().requires_grad_(), b0.detach().requires_grad_()
+        xh = x.permute(0, 2, 3, 1)
+        x8 = act8.pack(xh)
+        y = dconv.DConvAct8Fn.apply(xh, act8.Carrier.apply(xh), x8.codes, x8.exps, w, b, 3, 1, 1).permute(0, 3, 1, 2)
+        gx, gw, gb = torch.autograd.grad(y, (x, w, b), gy, create_graph=True)
+        return (y.detach(), gx.detach(), gw.detach()) + torch.autograd.grad((gx * u).sum() + gw.sum(), (x, gy, w))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*static)
+    for k in range(3):
+        new = [mk(64) * (k + 1), mk(32), mk(64)]
+        want = step(*new)
+        for s, n in zip(static, new):
+            s.copy_(n)
+        graph.replay()
+        torch.cuda.synchronize()
+        for i, (p, q) in enumerate(zip(out, want)):
+            assert torch.equal(p, q), (i, shape)
+
+
+def test_offsets_past_31_bits(gpu_device):
+    """More than 2^31 values: the last ones are packed, read, normalised and multiplied like the first."""
+    x = torch.randn(3, 3400, 3400, 64, device=gpu_device)
+    assert x.numel() > 2 ** 31
+    q = act8.pack(x)
+    last = act8.pack(x[2, -5:])
+    assert torch.equal(q.codes[2, -5:], last.codes) and torch.equal(q.exps[2, -5:], last.exps)
+    assert torch.equal(act8.Act8(q.codes[2, -5:], q.exps[2, -5:], 64).unpack(), last.unpack())
+    v = q.unpack()
+    assert torch.equal(v[2, -5:], last.unpack())
+    del v
+    with torch.no_grad():
+        y = gn.group_norm_lrelu(x.permute(0, 3, 1, 2), 32)[2, :, -4:].clone()
+        y1 = gn.group_norm_lrelu(x[2:].permute(0, 3, 1, 2), 32)[0, :, -4:]
+    torch.testing.assert_close(y, y1, rtol=2 ** -22, atol=1e-9)  # the sums' order differs: 1e-16 of the statistics
+    del x
+    gy = torch.randn(3, 3400, 3400, 4, device=gpu_device)
+    whole = dconv.conv_wgrad_act8(q, gy, 1, 1, 0)
+    parts = sum(dconv.conv_wgrad_act8(act8.Act8(q.codes[i:i + 1], q.exps[i:i + 1], 64), gy[i:i + 1], 1, 1, 0).double()
+                for i in range(3))
+    # sums of 3.5e7 products in float32, of order sqrt(3.5e7): 2^-24 of a partial sum per addition of a 256-way split
+    torch.testing.assert_close(whole.double(), parts, rtol=0, atol=2 ** -24 * (3.5e7 / 256) ** 0.5 * 5900)
+
+
 def _disc(g, norm, ck, seed=0):
     torch.manual_seed(seed)
     netD = Discriminator_VGG_128_(3, 64, norm_type=norm, nb=6, num_2_strides=3, act_checkpoint=ck)
@@ -315,3 +377,37 @@ def test_carrier_adds_nothing_to_a_first_backward(gpu_device):
         torch.autograd.grad(y, x, gy)
     names = {e.name for e in prof.events()}
     assert not names & {'aten::zeros', 'aten::fill_', 'aten::add', 'aten::add_', 'aten::copy_'}, names
+
+
+@pytest.mark.parametrize('norm,ck', [('group', None), ('group', 'int8'), ('instance', 'int8'), ('batch', 'int8')])
+def test_training_loop_and_checkpoint_files(gpu_device, tmp_path, norm, ck):
+    """SRRaGANModel trains the discriminator with these options (both optimisers step, losses finite), writes it and
+    reads it back bit for bit."""
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), 'golden'))
+    from train_recipe import TRAIN_CFGS, step_data, train_opt
+    from esr_amd.SRRaGAN_model import SRRaGANModel
+    cfg = dict(TRAIN_CFGS['adaptive_rel'], D_update_ratio=1, D_valid_steps=1, min_D_prob_ratio_4_G=0.0,
+               min_mean_D_correct=-1.0)
+    opt = train_opt(cfg)
+    opt['network_D'].update(norm_type=norm, act_checkpoint=ck)
+    torch.manual_seed(3)
+    model = SRRaGANModel(opt, accumulation_steps_per_batch=1, device=gpu_device)
+    before = {k: v.detach().clone() for k, v in model.netD.named_parameters()}
+    for k in range(3):
+        lr, hr, z = (torch.from_numpy(a).to(gpu_device) for a in step_data(cfg, k))
+        model.feed_data({'LR': lr, 'HR': hr, 'Z': z})
+        model.optimize_parameters()
+    for key in ('l_d_gp', 'l_d_real_fake', 'D_real'):
+        if key in model.log_dict:
+            assert np.isfinite(np.asarray(model.log_dict[key], dtype=np.float64)).all(), key
+    moved = [k for k, v in model.netD.named_parameters() if not torch.equal(v, before[k])]
+    weights = [k for k in before if k.endswith('weight')]
+    assert set(weights) <= set(moved)
+    path = model.save_network(str(tmp_path), model.netD, 'D', 1, model.optimizer_D)
+    state = {k: v.detach().clone() for k, v in model.netD.state_dict().items()}
+    with torch.no_grad():
+        for p in model.netD.parameters():
+            p.zero_()
+    model.load_network(path, model.netD, optimizer=model.optimizer_D)
+    for k, v in model.netD.state_dict().items():
+        assert torch.equal(v, state[k]), k
