@@ -2,9 +2,10 @@
 //
 // A block is 32 consecutive channels of one pixel (the last block of a pixel may be shorter).  Its values share one
 // power-of-two step 2^(e - 132), e in [0, 254], the smallest with 127·step >= max|x|; a value is code·step, code in
-// [-127, 127] ([-63, 63] at e = 254).  A power of two because code·step is then exact in fp32 (and, with 7 significant bits, in f16 / bf16,
-// which is what the matrix-core weight gradient multiplies), and code = rint(x / step) has no division error: max error
-// step/2 <= max|x|/127.  e = 255 marks a block that holds an infinity or a NaN: all of it reads back as NaN.
+// [-127, 127] ([-63, 63] at e = 254).  A power of two because code·step is then exact in fp32 (and, with 7 significant
+// bits, in f16 / bf16, which is what the matrix-core weight gradient multiplies), and code = rint(x / step) has no
+// division error: max error step/2 <= max|x|/127, a whole step where a code is moved to keep x's side of a threshold.
+// e = 255 marks a block that holds an infinity or a NaN: all of it reads back as NaN.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -24,9 +25,9 @@ __device__ __forceinline__ int exp_of(unsigned amax_bits) {
     return q - 1 + ((amax_bits & 0x7fffffu) > 0x7e0000u ? 1 : 0);  // mantissa > 127/64: one power more
 }
 // (the largest step's codes stop at 63: 64 · 2^122 is past the largest float)
+__device__ __forceinline__ float most_of(int e) { return e == 254 ? 63.f : 127.f; }
 __device__ __forceinline__ float code_of(float x, int e) {
-    const float most = e == 254 ? 63.f : 127.f;
-    return e == 255 ? 0.f : fminf(fmaxf(rintf(ldexpf(x, 132 - e)), -most), most);
+    return e == 255 ? 0.f : fminf(fmaxf(rintf(ldexpf(x, 132 - e)), -most_of(e)), most_of(e));
 }
 __device__ __forceinline__ float value_of(float code, int e) {
     return e == 255 ? __builtin_nanf("") : ldexpf(code, e - 132);

@@ -305,7 +305,10 @@ __device__ __forceinline__ void put_blocks(const GnP &p, const float *v, bool ac
         float code = act8::code_of(v[k], e);
         if (act && e != 255) {
             const float at = act8::value_of(code, e);
-            if (pre(at, k) != pre(v[k], k)) code += at > v[k] ? -1.f : 1.f;
+            if (pre(at, k) != pre(v[k], k)) {
+                const float to = code + (at > v[k] ? -1.f : 1.f);
+                if (fabsf(to) <= act8::most_of(e)) code = to;  // (past the largest float there is no step to go)
+            }
         }
         w |= (uint32_t)(uint8_t)(int8_t)(int)code << (8 * k);
     }

@@ -2,9 +2,9 @@
 //   gw[co][ci][ky][kx] = Σ_{b, Y, X} x[b, s·Y + ky − p, s·X + kx − p, ci] · dy[b, Y, X, co]   (x zero outside the image)
 // One matrix product per tap, M = ci, N = co, K = output pixels, on v_mfma_f32_32x32x16_f16.  A code is an integer of 7
 // bits times a power of two, so x is ONE exact f16 number (at a scale of the workgroup's largest exponent; a block more
-// than 2^32 below it counts as zero), and only dy is split, into hi + lo f16 at a power-of-two scale of the largest |dy|
-// so far (|dy − hi − lo| <= 2^-22 |dy| + 2^-36 of that largest): two products where fp32 x takes three, and a quarter of
-// its bytes.  The scales leave room for a growth of 2^4 (dy) and 2^2 (x); a tile beyond that raises a flag, and the
+// than 2^27 below it counts as zero, a subnormal f16's sums round like those of 2^-14), and only dy is split, into hi +
+// lo f16 at a power-of-two scale of the largest |dy| so far (|dy − hi − lo| <= 2^-22 |dy| + 2^-36 of that largest): two
+// products where fp32 x takes three, and a quarter of its bytes.  The scales leave room for a growth of 2^4 (dy) and 2^2 (x); a tile beyond that raises a flag, and the
 // workgroup finds its maxima, rescales the float32 accumulators by the exact power of two and stages the tile again.
 //
 // A workgroup owns 64 ci × 64 co and ALL the taps of a tap group (3×3: nine; 4×4 stride 2: sixteen; 4×4 stride 1: two
@@ -38,6 +38,7 @@ struct WgP {
     const uint8_t *exps;
     const float *dy;
     int B, Hs, Ws, cin, cp, nb, MH, MW, cout, k, s, p, nci, nco, groups;
+    int Hr, Wr;                            // rows and columns of x that an output reads (non-finite ones behind them count not)
     int tY, tX, tiles, per_split, splits;  // K steps: rows and columns of tiles per image, all, per split
     float *partial;                        // [splits][k·k][nci·64][nco·64]
 };
@@ -113,8 +114,9 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
 #pragma unroll
         for (int j = 0; j < H::NX; ++j) {
             const int sy = ys + (xr[j] >> 16) * st, sx = xs + (xr[j] & 0xffff) * st, ci = ci0 + 16 * (tid & 3);
-            const bool in = xr[j] >= 0 && (unsigned)sy < (unsigned)p.Hs && (unsigned)sx < (unsigned)p.Ws;
-            const unsigned m = -(unsigned)in, pix = (unsigned)(sy * p.Ws + sx) & m, c = (unsigned)ci & m;  // (no branch)
+            const bool in = xr[j] >= 0 && (unsigned)sy < (unsigned)p.Hr && (unsigned)sx < (unsigned)p.Wr;
+            // (no branch; unsigned, for the places outside are computed too)
+            const unsigned m = -(unsigned)in, pix = ((unsigned)sy * p.Ws + sx) & m, c = (unsigned)ci & m;
             ok |= (int)in << j;
             re[j] = exps[pix * (unsigned)p.nb + c / act8::BLK];
             rx[j] = *reinterpret_cast<const uint4 *>(codes + (pix * (unsigned)p.cp + c));
@@ -323,8 +325,9 @@ __global__ __launch_bounds__(NT) void wgrad8_reduce(const float *partial, int sp
     }
 }
 
-// The same for many weights (and so few splits): a workgroup adds 32 co × cb ci × all taps (at most 64 of the latter two) and
-// writes them by rows of one co, which lie together in gw (one by one, at a stride of cin·T, each would cost a sector).
+// The same for many weights (and so few splits): a workgroup adds 32 co × cb ci × all taps (at most 64 of the latter two)
+// and writes them by rows of one co, which lie together in gw (one by one, at a stride of cin·T, each would cost a
+// sector).
 __global__ __launch_bounds__(NT) void wgrad8_reduce_rows(const float *partial, int splits, int T, int cin, int cout, int cip,
                                                          int cop, int cb, float *gw) {
     __shared__ float tile[32][65];
@@ -358,12 +361,19 @@ bool geometry(int64_t B, int32_t Hs, int32_t Ws, int32_t cin, int32_t MH, int32_
     if (Hs + 2 * pad < k || Ws + 2 * pad < k) return false;
     if (MH != (Hs + 2 * pad - k) / s + 1 || MW != (Ws + 2 * pad - k) / s + 1) return false;
     // (offsets within an image are 32-bit)
-    if ((int64_t)MH * MW > 0x7fffffffLL / cout / 4 || (int64_t)Hs * Ws > 0x7fffffffLL / act8::pitch(cin) || B > 0x7fffffff) return false;
+    if ((int64_t)MH * MW > 0x7fffffffLL / cout / 4 || (int64_t)Hs * Ws > 0x7fffffffLL / act8::pitch(cin)) return false;
+    if (B > 0x7fffffff) return false;
     g.kind = k == 3 && s == 1 ? 0 : k == 4 && s == 2 ? 1 : k == 4 && s == 1 ? 2 : k == 8 && s == 1 ? 3 : 4;
     WgP &p = g.p;
     p = WgP{};
-    p.B = (int)B; p.Hs = Hs; p.Ws = Ws; p.cin = cin; p.cp = act8::pitch(cin); p.nb = (cin + 31) / 32; p.MH = MH; p.MW = MW; p.cout = cout;
-    p.k = k; p.s = s; p.p = pad;
+    p.B = (int)B; p.Hs = Hs; p.Ws = Ws; p.cin = cin; p.cp = act8::pitch(cin); p.nb = (cin + 31) / 32;
+    p.MH = MH; p.MW = MW; p.cout = cout; p.k = k; p.s = s; p.p = pad;
+    auto read = [&](int size, int out) {
+        const int n = (out - 1) * s + k - pad;
+        return n < 0 ? 0 : n < size ? n : size;
+    };
+    p.Hr = read(Hs, MH);
+    p.Wr = read(Ws, MW);
     p.nci = (cin + 63) / 64;
     p.nco = (cout + 63) / 64;
     p.groups = g.kind <= 1 ? 1 : g.kind == 2 ? 2 : g.kind == 3 ? 8 : k * k;
@@ -416,7 +426,9 @@ extern "C" int esr_dconv_wgrad_act8(const int8_t *codes, const uint8_t *exps, in
                                     int32_t cin, const float *dy, int32_t MH, int32_t MW, int32_t cout, int32_t k,
                                     int32_t s, int32_t pad, float *gw, void *ws, esr_stream_t stream) {
     Geo g;
-    if (!codes || !exps || !dy || !gw || !ws || (uintptr_t)codes % 16 || (uintptr_t)ws % 16 || !geometry(B, Hs, Ws, cin, MH, MW, cout, k, s, pad, g)) return ESR_EINVAL;
+    if (!codes || !exps || !dy || !gw || !ws || (uintptr_t)codes % 16 || (uintptr_t)ws % 16 ||
+        !geometry(B, Hs, Ws, cin, MH, MW, cout, k, s, pad, g))
+        return ESR_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
     WgP &p = g.p;
     p.codes = codes; p.exps = exps; p.dy = dy; p.partial = (float *)ws;

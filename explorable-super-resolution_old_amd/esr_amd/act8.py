@@ -2,7 +2,8 @@
 
 A training step of the discriminator keeps every convolution's input and every norm's input until the backward reads
 them: 8 bytes per activation value in fp32.  `pack` keeps 1 + 1/32: int8 codes that share a power-of-two step per 32
-channels of a pixel (error <= half a step <= max|x|/127 of the block; x > 0 is kept exactly, so LeakyReLU masks are).
+channels of a pixel (error <= half a step <= max|x|/127 of the block; x > 0 is kept exactly, so LeakyReLU masks are: a
+positive value below half a step takes code 1).
 The backward kernels read the codes themselves: dconv.conv_wgrad_act8 (weight gradients) and gn.group_norm_lrelu
 (checkpoint='int8')."""
 import contextlib

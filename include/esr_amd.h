@@ -463,14 +463,16 @@ int esr_bn_lrelu_bwd2(const float *x, const float *gy, const float *u, const flo
 /* ---- activations kept in 8 bits (esr_act8.hip, esr_wgrad8.hip) ------------------------------------------------------
  * What the discriminator's blocks keep of an activation x [P][C] (P pixels, channels last) from the forward to the
  * backward pass: codes int8 [P][16 * ceil(C / 16)] (16-byte aligned; 0 behind channel C), and one exponent byte per 32
- * channels of a pixel, exps [P][ceil(C / 32)]; the value
- * of a code is code · 2^(e − 132), e the smallest with 127 · 2^(e − 132) >= the block's max |x| (e = 255: the block
- * holds an infinity or a NaN and reads back as NaN).  Error <= half a step <= max|x|/127; x > 0 is kept exactly (a
- * positive value never takes code 0).  C need not be a multiple of 32 or of 4.
+ * channels of a pixel, exps [P][ceil(C / 32)]; the value of a code is code · 2^(e − 132), e the smallest with
+ * 127 · 2^(e − 132) >= the block's max |x| (e = 255: the block holds an infinity or a NaN and reads back as NaN).
+ * Error <= half a step <= max|x|/127; x > 0 is kept exactly (a positive value never takes code 0: less than a step).
+ * C need not be a multiple of 32 or of 4.
  * esr_dconv_wgrad_act8: the weight gradient of conv2d(x, w, stride s, zero padding pad) from x's blocks:
  *   gw[co][ci][ky][kx] = sum over b, Y, X of x[b, s*Y + ky - pad, s*X + kx - pad, ci] * dy[b, Y, X, co]
  * x [B][Hs][Ws][cin], dy [B][MH][MW][cout] fp32, MH = (Hs + 2·pad − k) / s + 1 (likewise MW), k <= 8, gw in torch's
  * layout; ws = esr_dconv_wgrad_act8_workspace_bytes(...) bytes, 16-byte aligned (ESR_EINVAL on bad arguments).
+ * Sizes: Hs, Ws <= 65535, cin, cout <= 65536, an image's codes and four times its dy's values < 2^31 (ESR_EINVAL).  A
+ * non-finite block makes the weights of its channels non-finite at every tap, a non-finite dy those of its output.
  * Deterministic. */
 int esr_act8_pack(const float *x, int64_t P, int32_t C, int8_t *codes, uint8_t *exps, esr_stream_t stream);
 int esr_act8_unpack(const int8_t *codes, const uint8_t *exps, int64_t P, int32_t C, float *x, esr_stream_t stream);
@@ -482,9 +484,10 @@ int esr_dconv_wgrad_act8(const int8_t *codes, const uint8_t *exps, int64_t B, in
 
 /* ---- GroupNorm + LeakyReLU, channels last (esr_gn.hip) -------------------------------------------------------------
  * x, y, gy, ... [N][HW][C] fp32; G groups of C/G channels; gamma, beta [C] or NULL (1, 0; G = C without them is
- * instance norm).  y = lrelu_slope(γ·(x − μ)·r + β), r = 1/sqrt(v + eps) over each (sample, group).
+ * instance norm); N <= 65535, C <= 2^24.  y = lrelu_slope(γ·(x − μ)·r + β), r = 1/sqrt(v + eps) over each (sample, group).
  * esr_gn_lrelu_fwd writes y and stat [N][G][2] (μ and r, float64) and, where codes / exps are given, x in 8-bit
- *   blocks (above) whose pre-activations keep the sign x's have (a code moves one step where rounding would change it);
+ *   blocks (above) whose pre-activations keep the sign x's have (a code moves one step where rounding would change it,
+ *   so that its error is less than a step; at e = 254 it stays where that step leads past the largest float);
  *   where ycodes / yexps are given, y's blocks as esr_act8_pack's.
  * esr_gn_lrelu_bwd: gx, g_gamma, g_beta (each may be NULL) for upstream gy, and sums [N][2][C] (float64:
  *   Σ gz, Σ gz·x̂ per sample and channel).  The input is x, or codes / exps with x NULL.

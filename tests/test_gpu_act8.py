@@ -126,6 +126,25 @@ def test_wgrad_ranges(gpu_device, kind):
     check_wgrad(gpu_device, x, gy, 3, 1, 1)
 
 
+@pytest.mark.parametrize('below', [0, 11, 16, 20, 24, 27])
+def test_wgrad_of_blocks_far_below_the_largest(gpu_device, below):
+    """A block's codes are exact down to 2^-27 of the workgroup's largest: where only that block's pixel has a gradient,
+    the weights are its values times the gradient."""
+    x = np.zeros((1, 1, 2, 32), np.float32)
+    x[0, 0, 0] = np.arange(32) * 4 + 3
+    x[0, 0, 1] = (np.arange(32) * 4 + 3) * np.float32(2.0 ** -below)
+    gy = np.zeros((1, 1, 2, 64), np.float32)
+    gy[0, 0, 1] = np.linspace(-1.3, 1.7, 64)
+    got = dconv.conv_wgrad_act8(act8.pack(torch.from_numpy(x).to(gpu_device)), torch.from_numpy(gy).to(gpu_device), 1, 1,
+                                0).double().cpu().numpy()[:, :, 0, 0]
+    want = np.outer(gy[0, 0, 1].astype(np.float64), x[0, 0, 1].astype(np.float64))
+    # The gradient's two pieces (2^-22 of it + 2^-36 of the largest, 2) and two additions' roundings.  Those of an x that
+    # is a subnormal f16 are 2^-24 of the product that f16's least exponent gives: x is staged at 8 times its value here
+    # (step 1, scale 2^3), so of 2^-13 / 8 times the gradient's next power of two, twice: 2 · 2^-24 · 2^-16 · 2 |gy|.
+    sub = 2.0 ** -38 * np.abs(gy[0, 0, 1].astype(np.float64))[:, None]
+    assert (np.abs(got - want) <= 2.0 ** -21 * np.abs(want) + 2.0 ** -35 * np.abs(x[0, 0, 1]) + sub).all()
+
+
 @pytest.mark.parametrize('where', ['x', 'gy'])
 def test_wgrad_nonfinite(gpu_device, where):
     """A NaN reaches the weights that it belongs to: its block's input channels, or its output channel."""
@@ -142,6 +161,20 @@ def test_wgrad_nonfinite(gpu_device, where):
         assert bad[:, 32:].all() and not bad[:, :32].any()
     else:
         assert bad[65].all() and not bad[:65].any() and not bad[66:].any()
+
+
+@pytest.mark.parametrize('geo', [(1, 8, 9, 32, 64, 3, 2, 0), (2, 7, 9, 64, 40, 4, 2, 0), (1, 12, 30, 33, 8, 2, 5, 0),
+                                 (1, 3, 3, 8, 8, 1, 100, 5)])
+def test_wgrad_of_pixels_that_no_output_reads(gpu_device, geo):
+    """Infinities in rows and columns that the strides leave unread do not reach the weights."""
+    B, H, W, Ci, Co, k, s, p = geo
+    x, gy = wgrad_case(geo, 9)
+    want = check_wgrad(gpu_device, x, gy, k, s, p)
+    rows, cols = (max(0, (dconv.out_size(n, k, s, p) - 1) * s + k - p) for n in (H, W))
+    assert rows < H or cols < W
+    x[:, rows:], x[:, :, cols:] = np.inf, np.nan
+    got = dconv.conv_wgrad_act8(act8.pack(torch.from_numpy(x).to(gpu_device)), torch.from_numpy(gy).to(gpu_device), k, s, p)
+    assert np.array_equal(got.double().cpu().numpy(), want)
 
 
 def test_wgrad_refusals(gpu_device):

@@ -163,6 +163,25 @@ def test_masks_of_blocks_are_the_forwards(gpu_device, ck):
         assert torch.equal(gb, want.sum((0, 2, 3)).float())
 
 
+def test_blocks_next_to_the_largest_float(gpu_device):
+    """The kink between the largest code's value, 63/64 · 2^128, and the largest float: no code on the float's side of it
+    is finite, so the largest one stays (x̂ = 0.97 of ±1 with β = −0.98), and the gradients stay finite."""
+    top = float(np.finfo(np.float32).max)
+    for W in (2, 4096):  # one launch, three launches
+        x = torch.zeros(1, 32, 64, W, device=gpu_device).contiguous(memory_format=torch.channels_last)
+        x[..., W // 2:] = top
+        x.requires_grad_()
+        w = torch.ones(32, device=gpu_device, requires_grad=True)
+        b = torch.full((32,), -0.98, device=gpu_device, requires_grad=True)
+        y, y8 = gn.group_norm_lrelu(x, 32, w, b, 1e-5, 0.25, 'int8', out8=True)
+        assert torch.isfinite(y).all() and torch.isfinite(y8.unpack()).all()
+        # x̂ is −1 and 0.96875 at the codes' values, both on the slope's side
+        _, gw, gb = torch.autograd.grad(y.sum(), (x, w, b))
+        half = 64 * W // 2
+        assert torch.equal(gb, torch.full_like(gb, 0.25 * 2 * half))
+        assert torch.allclose(gw, torch.full_like(gw, 0.25 * half * -0.03125), rtol=1e-5, atol=0)
+
+
 def test_layouts_and_offsets(gpu_device):
     """NCHW storage, channel slices, transposed maps and bases off 16 bytes give the channels-last result bit for bit."""
     c = R.case((2, 24, 6, 5), 4, seed=4, dtype=np.float32)
