@@ -26,14 +26,13 @@ __device__ __forceinline__ uint32_t codes_of(const float *v, int &e) {
 #pragma unroll
     for (int k = 0; k < V; ++k) m = max(m, act8::abs_bits(v[k]));
     e = act8::exp_of(act8::block_max<act8::BLK / V>(m));
-    uint32_t w = 0;
+    float code[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        float code = act8::code_of(v[k], e);
-        if (e != 255 && code == 0.f && v[k] > 0.f) code = 1.f;
-        w |= (uint32_t)(uint8_t)(int8_t)(int)code << (8 * k);
+        code[k] = act8::code_of(v[k], e);
+        code[k] = v[k] > 0.f ? fmaxf(code[k], 1.f) : code[k];
     }
-    return w;
+    return act8::word_of<V>(code, e);
 }
 
 template <int V>

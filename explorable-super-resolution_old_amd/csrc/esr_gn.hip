@@ -289,29 +289,25 @@ __global__ __launch_bounds__(NT) void gn_finish(GnP p, const double *partial, do
     results<MODE>(p, n, g0 + tid, t, out + S::O * ((long long)n * p.G + g0 + tid));
 }
 
-// codes of V values of one row in a block whose lanes call together; pre: z of a value
+// codes of V values of one row in a block whose lanes call together; up: their sides of the threshold, side: a value's
 template <int V, typename F>
-__device__ __forceinline__ void put_blocks(const GnP &p, const float *v, bool act, long long row, int c, int lane,
-                                           int8_t *codes, uint8_t *exps, F pre) {
+__device__ __forceinline__ void put_blocks(const GnP &p, const float *v, const bool *up, bool act, long long row, int c,
+                                           int lane, int8_t *codes, uint8_t *exps, F side) {
     constexpr int L = act8::BLK / V;
     unsigned m = 0;
 #pragma unroll
     for (int k = 0; k < V; ++k) m = max(m, act8::abs_bits(v[k]));
     const int e = act8::exp_of(act8::block_max<L>(m));
     if (c >= p.cp) return;  // (behind the last channel the code is 0)
-    uint32_t w = 0;
+    float code[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        float code = act8::code_of(v[k], e);
-        if (act && e != 255) {
-            const float at = act8::value_of(code, e);
-            if (pre(at, k) != pre(v[k], k)) {
-                const float to = code + (at > v[k] ? -1.f : 1.f);
-                if (fabsf(to) <= act8::most_of(e)) code = to;  // (past the largest float there is no step to go)
-            }
-        }
-        w |= (uint32_t)(uint8_t)(int8_t)(int)code << (8 * k);
+        const float to = act8::code_of(v[k], e), at = ldexpf(to, e - 132);
+        // (past the largest float there is no step to go)
+        const float back = act8::keep(to + (at > v[k] ? -1.f : 1.f), e);
+        code[k] = act & (side(at, k) != up[k]) ? back : to;
     }
+    const uint32_t w = act8::word_of<V>(code, e);
     if constexpr (V == 4) *reinterpret_cast<uint32_t *>(codes + row * p.cp + c) = w;
     else codes[row * p.cp + c] = (int8_t)w;
     if (lane % L == 0) exps[row * p.nb + c / act8::BLK] = (uint8_t)e;
@@ -353,6 +349,7 @@ __device__ __forceinline__ void apply_of(const GnP &p, const GnOut &o, const Cha
     const int tid = threadIdx.x, lane = tid % p.lanes, ph = tid / p.lanes;
     const int c = chunk * p.step + lane * V;
     const bool act = c < min(p.C, (chunk + 1) * p.step);
+    const int cl = act ? c : chunk * p.step;
     if (ph >= p.rpi) return;
     float k0[V], k1[V], k3[V], k4[V], k5[V], k6[V], ua[V], ub[V];
     if (act) {
@@ -376,43 +373,41 @@ __device__ __forceinline__ void apply_of(const GnP &p, const GnOut &o, const Cha
     for (long long q = r0 + ph; q < r1; q += UA * p.rpi) {
         Raw<V, Q8> raw[UA];
         float gy[UA][V], u[UA][V];
-        if (act) {
 #pragma unroll
-            for (int j = 0; j < UA; ++j) {
-                const long long row = (long long)n * p.HW + min(q + j * p.rpi, r1 - 1);
-                raw[j].load(p, row, c);
-                if constexpr (MODE >= 1) load_f<V>(p.gy, row * p.C + c, gy[j]);
-                if constexpr (MODE == 2) {
-                    if (p.u) load_f<V>(p.u, row * p.C + c, u[j]);
-                    else
+        for (int j = 0; j < UA; ++j) {  // (lanes behind the last channel load the chunk's first)
+            const long long row = (long long)n * p.HW + min(q + j * p.rpi, r1 - 1);
+            raw[j].load(p, row, cl);
+            if constexpr (MODE >= 1) load_f<V>(p.gy, row * p.C + cl, gy[j]);
+            if constexpr (MODE == 2) {
+                if (p.u) load_f<V>(p.u, row * p.C + cl, u[j]);
+                else
 #pragma unroll
-                        for (int v = 0; v < V; ++v) u[j][v] = 0.f;
-                }
+                    for (int v = 0; v < V; ++v) u[j][v] = 0.f;
             }
         }
-#pragma unroll
-        for (int j = 0; j < UA; ++j) {
-            if (q + j * p.rpi >= r1) break;
+        auto finish = [&](int j) {
             const long long row = (long long)n * p.HW + q + j * p.rpi;
             float a[V], d[V];
-            if (act) {
+            bool up[V];
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const double xd = xhat(raw[j].at(v), ch.r[v], ch.mu[v]), z = preact(xd, ch.ga[v], ch.be[v]);
-                    if constexpr (MODE == 0) {
-                        a[v] = (float)(z * (z > 0.0 ? 1.0 : (double)p.slope));
+            for (int v = 0; v < V; ++v) {
+                const double xd = xhat(raw[j].at(v), ch.r[v], ch.mu[v]), z = preact(xd, ch.ga[v], ch.be[v]);
+                if constexpr (MODE == 0) {
+                    up[v] = z > 0.0;
+                    a[v] = (float)(z * (up[v] ? 1.0 : (double)p.slope));
+                } else {
+                    const float m = z > 0.0 ? 1.f : p.slope, xh = (float)xd, rf = (float)ch.r[v], gf = (float)ch.ga[v];
+                    const float gz = gy[j][v] * m, h = gf * gz;
+                    if constexpr (MODE == 1) {
+                        a[v] = rf * (h - k0[v] - xh * k1[v]);
                     } else {
-                        const float m = z > 0.0 ? 1.f : p.slope, xh = (float)xd, rf = (float)ch.r[v], gf = (float)ch.ga[v];
-                        const float gz = gy[j][v] * m, h = gf * gz;
-                        if constexpr (MODE == 1) {
-                            a[v] = rf * (h - k0[v] - xh * k1[v]);
-                        } else {
-                            const float uu = u[j][v], gg = -rf * (h * k1[v] + uu * k3[v]) + ua[v] * gz;
-                            d[v] = m * (gf * rf * (uu - k0[v] - xh * k1[v]) + ua[v] * xh + ub[v]);
-                            a[v] = rf * (gg - k4[v] - xh * k5[v]) - k6[v] * xh;
-                        }
+                        const float uu = u[j][v], gg = -rf * (h * k1[v] + uu * k3[v]) + ua[v] * gz;
+                        d[v] = m * (gf * rf * (uu - k0[v] - xh * k1[v]) + ua[v] * xh + ub[v]);
+                        a[v] = rf * (gg - k4[v] - xh * k5[v]) - k6[v] * xh;
                     }
                 }
+            }
+            if (act) {
                 store_f<V>(o.o1, row * p.C + c, a);
                 if constexpr (MODE == 2) store_f<V>(o.o2, row * p.C + c, d);
             }
@@ -424,12 +419,24 @@ __device__ __forceinline__ void apply_of(const GnP &p, const GnOut &o, const Cha
                     a[v] = act ? a[v] : 0.f;
                 }
                 if (o.codes)
-                    put_blocks<V>(p, t, act, row, c, lane, o.codes, o.exps, [&](float x, int v) {
+                    put_blocks<V>(p, t, up, act, row, c, lane, o.codes, o.exps, [&](float x, int v) {
                         return preact(xhat(x, ch.r[v], ch.mu[v]), ch.ga[v], ch.be[v]) > 0.0;
                     });
-                if (o.ycodes)
-                    put_blocks<V>(p, a, act, row, c, lane, o.ycodes, o.yexps, [](float y, int) { return y > 0.f; });
+                if (o.ycodes) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) up[v] = a[v] > 0.f;
+                    put_blocks<V>(p, a, up, act, row, c, lane, o.ycodes, o.yexps, [](float y, int) { return y > 0.f; });
+                }
             }
+        };
+        // (all of the rows without a branch between them, so that they overlap; but for a workgroup's last ones)
+        if (q + (UA - 1) * p.rpi < r1) {
+#pragma unroll
+            for (int j = 0; j < UA; ++j) finish(j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < UA - 1; ++j)
+                if (q + j * p.rpi < r1) finish(j);
         }
     }
 }
