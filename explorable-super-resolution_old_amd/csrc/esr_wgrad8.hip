@@ -4,8 +4,9 @@
 // bits times a power of two, so x is ONE exact f16 number (at a scale of the workgroup's largest exponent; a block more
 // than 2^27 below it counts as zero, a subnormal f16's sums round like those of 2^-14), and only dy is split, into hi +
 // lo f16 at a power-of-two scale of the largest |dy| so far (|dy − hi − lo| <= 2^-22 |dy| + 2^-36 of that largest): two
-// products where fp32 x takes three, and a quarter of its bytes.  The scales leave room for a growth of 2^4 (dy) and 2^2 (x); a tile beyond that raises a flag, and the
-// workgroup finds its maxima, rescales the float32 accumulators by the exact power of two and stages the tile again.
+// products where fp32 x takes three, and a quarter of its bytes.  The scales leave room for a growth of 2^4 (dy) and 2^2
+// (x); a tile beyond that raises a flag, and the workgroup finds its maxima, rescales the float32 accumulators by the
+// exact power of two and stages the tile again.
 //
 // A workgroup owns 64 ci × 64 co and ALL the taps of a tap group (3×3: nine; 4×4 stride 2: sixteen; 4×4 stride 1: two
 // rows; 8×8: one row), a wave one 32×32 tile for each of up to nine taps: dy is expanded once per K step for all of
@@ -301,26 +302,26 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
             dst[((long long)t * cip + (r & 3) + 8 * (r >> 2) + 4 * hl) * cop] = ldexpf(acc[t][r], back);
 }
 
-// gw[co][ci][t] = Σ over the splits: 32 consecutive co (four to a thread) × 32 slices of the splits, a slice in order,
-// then the slices
+// gw[co][ci][t] = Σ over the splits: 64 consecutive co (four to a thread: 256 bytes together) × 16 slices of the splits,
+// a slice in order, then the slices.  (256 splits of 9×64×128 sums, 75 MB: 13 us; 32 co × 32 slices took 15.)
 __global__ __launch_bounds__(NT) void wgrad8_reduce(const float *partial, int splits, int T, int cin, int cout, int cip,
                                                     int cop, float *gw) {
-    __shared__ f32x4 sl[32][8];
-    const int q = threadIdx.x >> 3, o = threadIdx.x & 7, nco = (cout + 31) / 32;
-    const int co = blockIdx.x % nco * 32, row = blockIdx.x / nco, ci = row % cin, t = row / cin;
+    __shared__ f32x4 sl[16][16];
+    const int q = threadIdx.x >> 4, o = threadIdx.x & 15, nco = (cout + 63) / 64;
+    const int co = blockIdx.x % nco * 64, row = blockIdx.x / nco, ci = row % cin, t = row / cin;
     const long long step = (long long)T * cip * cop;
     const float *src = partial + ((long long)t * cip + ci) * cop + co + 4 * o;  // (cop is a multiple of 64)
-    const int s0 = splits * q / 32, s1 = splits * (q + 1) / 32;
+    const int s0 = splits * q / 16, s1 = splits * (q + 1) / 16;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int s = s0; s < s1; ++s) v += *reinterpret_cast<const f32x4 *>(src + s * step);
     sl[q][o] = v;
     __syncthreads();
-    if (threadIdx.x < 32 && co + (int)threadIdx.x < cout) {
+    if (threadIdx.x < 64 && co + (int)threadIdx.x < cout) {
         const float *col = reinterpret_cast<const float *>(sl) + threadIdx.x;
         float s = col[0];
 #pragma unroll
-        for (int r = 1; r < 32; ++r) s += col[32 * r];
+        for (int r = 1; r < 16; ++r) s += col[64 * r];
         gw[((long long)(co + threadIdx.x) * cin + ci) * T + t] = s;
     }
 }
@@ -440,7 +441,7 @@ extern "C" int esr_dconv_wgrad_act8(const int8_t *codes, const uint8_t *exps, in
         hipLaunchKernelGGL(wgrad8_reduce_rows, dim3((unsigned)rows), dim3(NT), 0, st, p.partial, p.splits, T, cin, cout,
                            p.nci * 64, p.nco * 64, cb, gw);
     else
-        hipLaunchKernelGGL(wgrad8_reduce, dim3((unsigned)nco * cin * T), dim3(NT), 0, st, p.partial, p.splits, T, cin, cout,
+        hipLaunchKernelGGL(wgrad8_reduce, dim3((unsigned)p.nco * cin * T), dim3(NT), 0, st, p.partial, p.splits, T, cin, cout,
                            p.nci * 64, p.nco * 64, gw);
     return hipGetLastError() == hipSuccess ? ESR_OK : ESR_ELAUNCH;
 }
