@@ -141,9 +141,7 @@ __device__ __forceinline__ void sums_of(const GnP &p, const Chan<V> &ch, int n, 
                 if constexpr (MODE >= 1) load_f<V>(p.gy, row * p.C + c, gy[j]);
                 if constexpr (MODE == 2) load_f<V>(p.u, row * p.C + c, u[j]);
             }
-#pragma unroll
-            for (int j = 0; j < UN; ++j) {
-                if (q + j * p.rpi >= r1) break;
+            const auto add = [&](int j) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     const double x = raw[j].at(v);
@@ -164,6 +162,14 @@ __device__ __forceinline__ void sums_of(const GnP &p, const Chan<V> &ch, int n, 
                         }
                     }
                 }
+            };
+            if (q + (UN - 1) * p.rpi < r1) {
+#pragma unroll
+                for (int j = 0; j < UN; ++j) add(j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < UN - 1; ++j)
+                    if (q + j * p.rpi < r1) add(j);
             }
         }
     }
@@ -243,29 +249,34 @@ struct Sizes {
 // A workgroup per sample and set of whole groups (32 channels' worth, or one larger group): the splits' sums per channel
 // (sums_out [n][K][C], or null), then each group's results (partial null: no upstream of gx).
 template <int MODE>
-__global__ __launch_bounds__(NT) void gn_finish(GnP p, const double *partial, double *sums_out, double *out) {
+__global__ __launch_bounds__(NTS) void gn_finish(GnP p, const double *partial, double *sums_out, double *out) {
     using S = Sizes<MODE>;
-    __shared__ double part[8][S::K][32], chan[S::J][33], tot[S::J][32];
+    constexpr int W = NTS / 64;
+    __shared__ double part[W][S::K][32], chan[S::J][33], tot[S::J][32];
     const int tid = threadIdx.x, lane = tid & 31, sl = tid >> 5, n = blockIdx.y;
     const int gpb = sets(p.Cg), g0 = blockIdx.x * gpb, ng = min(gpb, p.G - g0), c1 = (g0 + ng) * p.Cg;
-    for (int i = tid; i < S::J * 32; i += NT) tot[i / 32][i % 32] = 0.0;
+    if (tid < S::J * 32) tot[tid / 32][tid % 32] = 0.0;
     for (int c0 = g0 * p.Cg; c0 < c1; c0 += 32) {
         const int c = c0 + lane;
         double s[S::K] = {};
         if (c < c1 && partial)
 #pragma unroll 4
-            for (int sp = sl; sp < p.splits; sp += 8)
+            for (int sp = sl; sp < p.splits; sp += 2 * W)
 #pragma unroll
                 for (int k = 0; k < S::K; ++k) s[k] += partial[(((long long)n * p.splits + sp) * S::K + k) * p.C + c];
 #pragma unroll
-        for (int k = 0; k < S::K; ++k) part[sl][k][lane] = s[k];
+        for (int k = 0; k < S::K; ++k) {
+            s[k] += __shfl_xor(s[k], 32);
+            if (!(sl & 1)) part[sl >> 1][k][lane] = s[k];
+        }
         __syncthreads();
         if (sl == 0 && c < c1) {
             double sh[S::J];
 #pragma unroll
             for (int k = 0; k < S::K; ++k) {
                 s[k] = part[0][k][lane];
-                for (int q = 1; q < 8; ++q) s[k] += part[q][k][lane];
+#pragma unroll
+                for (int q = 1; q < W; ++q) s[k] += part[q][k][lane];
                 if (sums_out) sums_out[((long long)n * S::K + k) * p.C + c] = s[k];
             }
             shares<MODE>(p, n, c, s, sh);
@@ -273,7 +284,7 @@ __global__ __launch_bounds__(NT) void gn_finish(GnP p, const double *partial, do
             for (int j = 0; j < S::J; ++j) chan[j][lane] = sh[j];
         }
         __syncthreads();
-        for (int i = tid; i < S::J * ng; i += NT) {  // channels of a group, in order
+        for (int i = tid; i < S::J * ng; i += NTS) {  // channels of a group, in order
             const int j = i / ng, g = i - j * ng, a = p.Cg <= 32 ? g * p.Cg : 0;
             const int b = p.Cg <= 32 ? a + p.Cg : min(32, c1 - c0);
             double t = tot[j][g];
@@ -589,7 +600,7 @@ void pass(GnP p, const GnOut &o, double *partial, double *sums_out, double *out,
     const int gpb = sets(p.Cg);
     if (reduce)
         hipLaunchKernelGGL((gn_sums<MODE, V, MODE && BITS>), dim3(p.splits, p.N, p.chunks), dim3(NT), 0, st, p, partial);
-    hipLaunchKernelGGL(gn_finish<MODE>, dim3((p.G + gpb - 1) / gpb, p.N), dim3(NT), 0, st, p, reduce ? partial : nullptr,
+    hipLaunchKernelGGL(gn_finish<MODE>, dim3((p.G + gpb - 1) / gpb, p.N), dim3(NTS), 0, st, p, reduce ? partial : nullptr,
                        sums_out, out);
     hipLaunchKernelGGL((gn_apply<MODE, V, BITS>), dim3(p.blocks, p.N, p.chunks), dim3(NT), 0, st, p, o);
 }
