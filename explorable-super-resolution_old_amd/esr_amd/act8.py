@@ -80,6 +80,13 @@ class Act8:
         self.codes = codes if codes.data_ptr() % 16 == 0 else codes.clone()
         self.exps, self.shape = exps.contiguous(), lead + (channels,)
 
+    @classmethod
+    def of(cls, codes, exps, shape):
+        """Blocks that this package has just written, without the checks."""
+        a = cls.__new__(cls)
+        a.codes, a.exps, a.shape = codes, exps, tuple(shape)
+        return a
+
     @property
     def nbytes(self):
         return self.codes.numel() + self.exps.numel()
@@ -103,13 +110,14 @@ def pack(x):
     check_dev('act8', x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError('act8.pack: a tensor [..., C], got %s' % (tuple(x.shape),))
-    x = x.detach().contiguous()
+    if not x.is_contiguous():
+        x = x.detach().contiguous()
     codes, exps = empty_blocks(x.shape, x.device)
     if x.numel():
         with on(x.device):
             _lib.check(_lib.load().esr_act8_pack(x.data_ptr(), x.numel() // x.shape[-1], x.shape[-1], codes.data_ptr(),
                                                  exps.data_ptr(), stream(x.device)), 'esr_act8_pack')
-    return Act8(codes, exps, x.shape[-1])
+    return Act8.of(codes, exps, x.shape)
 
 
 class Carrier(torch.autograd.Function):

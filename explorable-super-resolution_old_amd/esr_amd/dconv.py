@@ -15,6 +15,7 @@ HipConv2d takes/returns NCHW tensors with NHWC storage (torch.channels_last), wh
 There is no CPU path: a CPU tensor raises.
 """
 import ctypes
+import functools
 import os
 
 import torch
@@ -274,6 +275,14 @@ def conv_wgrad(x, gy, k, s, p, prec=None):
     return red.view(k, k, cin_pad, cout_pad)[:, :, :Ci, :Co].permute(3, 2, 0, 1).contiguous()
 
 
+@functools.lru_cache(maxsize=256)
+def _wgrad_act8_bytes(*geom):
+    n = int(_lib.load().esr_dconv_wgrad_act8_workspace_bytes(*geom))
+    if n < 0:
+        raise RuntimeError('esr_dconv_wgrad_act8_workspace_bytes failed with esr_status %d for %s' % (n, geom))
+    return n
+
+
 def conv_wgrad_act8(x8, gy, k, s, p):
     """conv_wgrad from an input kept in 8 bits: x8 = act8.Act8 of the NHWC input, gy NHWC [B][Ho][Wo][Co] fp32; exact
     products of the codes' values with gy to fp32 accuracy (csrc/esr_wgrad8.hip)."""
@@ -291,17 +300,14 @@ def conv_wgrad_act8(x8, gy, k, s, p):
     if B == 0:
         return gy.new_zeros(Co, Ci, k, k)
     gy = gy.contiguous()
-    lib = _lib.load()
-    geom = (k, s, p)
-    n = int(lib.esr_dconv_wgrad_act8_workspace_bytes(B, H, W, Ci, gy.shape[1], gy.shape[2], Co, *geom))
-    if n < 0:
-        raise RuntimeError('esr_dconv_wgrad_act8_workspace_bytes failed with esr_status %d' % n)
-    gw = torch.empty(Co, Ci, k, k, device=gy.device, dtype=torch.float32)
-    ws = torch.empty(n, device=gy.device, dtype=torch.uint8)
-    with act8.on(gy.device):
-        _lib.check(lib.esr_dconv_wgrad_act8(x8.codes.data_ptr(), x8.exps.data_ptr(), B, H, W, Ci, gy.data_ptr(),
-                                            gy.shape[1], gy.shape[2], Co, *geom, gw.data_ptr(), ws.data_ptr(),
-                                            act8.stream(gy.device)), 'esr_dconv_wgrad_act8')
+    geom = (B, H, W, Ci, *gy.shape[1:], k, s, p)
+    dev = gy.device
+    gw = torch.empty((Co, Ci, k, k), device=dev, dtype=torch.float32)
+    ws = torch.empty(_wgrad_act8_bytes(*geom), device=dev, dtype=torch.uint8)
+    with act8.on(dev):
+        _lib.check(_lib.load().esr_dconv_wgrad_act8(x8.codes.data_ptr(), x8.exps.data_ptr(), *geom[:4], gy.data_ptr(),
+                                                    *geom[4:], gw.data_ptr(), ws.data_ptr(), act8.stream(dev)),
+                   'esr_dconv_wgrad_act8')
     return gw
 
 
@@ -410,7 +416,7 @@ class WgradAct8Fn(torch.autograd.Function):
     def forward(ctx, carrier, gy, codes, exps, k, s, p, prec=None):
         ctx.save_for_backward(carrier, gy, codes, exps)
         ctx.geom = (k, s, p, prec)
-        return conv_wgrad_act8(act8.Act8(codes, exps, carrier.shape[3]), gy, k, s, p)
+        return conv_wgrad_act8(act8.Act8.of(codes, exps, carrier.shape), gy, k, s, p)
 
     @staticmethod
     def backward(ctx, ggw):
@@ -419,7 +425,7 @@ class WgradAct8Fn(torch.autograd.Function):
         ggw = ggw.contiguous()
         g_x = DgradFn.apply(gy, ggw, k, s, p, carrier.shape[1], carrier.shape[2], prec) \
             if ctx.needs_input_grad[0] else None
-        g_gy = DConvFn.apply(act8.Act8(codes, exps, carrier.shape[3]).unpack(), ggw, None, k, s, p, prec) \
+        g_gy = DConvFn.apply(act8.Act8.of(codes, exps, carrier.shape).unpack(), ggw, None, k, s, p, prec) \
             if ctx.needs_input_grad[1] else None
         return g_x, g_gy, None, None, None, None, None, None
 
@@ -527,7 +533,7 @@ def _df_bwd(xh, gy, mask, slope, w, need_x, need_w):
 
 def _df_mask(y, y8):
     """The layer's output, or its 8-bit values (their y > 0 is the output's) where it was kept so."""
-    return y if y8 is None else act8.Act8(*y8, 64).unpack()
+    return y if y8 is None else act8.Act8.of(*y8, y8[0].shape[:-1] + (64,)).unpack()
 
 
 class _DFirstFn(torch.autograd.Function):
@@ -628,7 +634,7 @@ def dfirst_lrelu8(x, conv, slope):
         xh = _ToNHWC.apply(x)
     if conv.keeps8():
         y, *y8 = _DFirstFn.apply(xh, conv.weight, conv.bias, float(slope), True)
-        return y.permute(0, 3, 1, 2), act8.Act8(*y8, 64)
+        return y.permute(0, 3, 1, 2), act8.Act8.of(*y8, y.shape)
     return _DFirstFn.apply(xh, conv.weight, conv.bias, float(slope)).permute(0, 3, 1, 2), None
 
 

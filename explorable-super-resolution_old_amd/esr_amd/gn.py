@@ -157,7 +157,7 @@ def group_norm_lrelu(x, groups, weight=None, bias=None, eps=1e-5, slope=0.2, che
     needs = checkpoint and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))
     out = _GNLReLUFn.apply(x, act8.Carrier.apply(x) if needs else None, weight, bias, int(groups), float(eps),
                            float(slope), bool(out8))
-    return (out[0], act8.Act8(*out[1:], C)) if out8 else out
+    return (out[0], act8.Act8.of(*out[1:], (B, H, W, C))) if out8 else out
 
 
 class HipGroupNorm(nn.GroupNorm):
