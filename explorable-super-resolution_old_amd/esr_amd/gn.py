@@ -70,11 +70,11 @@ class _GNLReLUFn(torch.autograd.Function):
         stat = torch.empty(2 * N * G, device=dev, dtype=torch.float64)
         codes, exps = act8.empty_blocks((N, H, W, C), dev) if carrier is not None else (None, None)
         y8 = act8.empty_blocks((N, H, W, C), dev) if out8 else (None, None)
+        ws = _bytes(_ws_bytes(N, H * W, C, G), dev)  # (held by its name until the launches are enqueued)
         with act8.on(dev):
             _lib.check(_lib.load().esr_gn_lrelu_fwd(x.data_ptr(), N, H * W, C, G, _p(gamma), _p(beta), eps, slope,
                                                     y.data_ptr(), stat.data_ptr(), _p(codes), _p(exps), _p(y8[0]),
-                                                    _p(y8[1]), _bytes(_ws_bytes(N, H * W, C, G), dev).data_ptr(),
-                                                    act8.stream(dev)), 'esr_gn_lrelu_fwd')
+                                                    _p(y8[1]), ws.data_ptr(), act8.stream(dev)), 'esr_gn_lrelu_fwd')
         ctx.save_for_backward(x if carrier is None else carrier, codes, exps, gamma, beta, stat)
         ctx.geom = (G, slope)
         if not out8:
@@ -119,12 +119,12 @@ class _GNLReLUBwdFn(torch.autograd.Function):
         g_gamma = torch.empty(C, device=dev, dtype=torch.float32) if gamma is not None else None
         ggx = None if ggx is None else _nhwc(ggx)
         ggg, ggb = (None if t is None else t.contiguous() for t in (ggg, ggb))
+        ws = _bytes(_ws_bytes(N, H * W, C, G), dev)
         with act8.on(dev):
             _lib.check(_lib.load().esr_gn_lrelu_bwd2(_p(src) if codes is None else None, _p(codes), _p(exps),
                                                      gy.data_ptr(), _p(ggx), _p(ggg), _p(ggb), N, H * W, C, G,
                                                      _p(gamma), _p(beta), stat.data_ptr(), slope, sums.data_ptr(),
-                                                     g_x.data_ptr(), g_gy.data_ptr(), _p(g_gamma),
-                                                     _bytes(_ws_bytes(N, H * W, C, G), dev).data_ptr(),
+                                                     g_x.data_ptr(), g_gy.data_ptr(), _p(g_gamma), ws.data_ptr(),
                                                      act8.stream(dev)), 'esr_gn_lrelu_bwd2')
         return g_x, g_gamma, None, g_gy, None, None, None, None, None
 
