@@ -32,10 +32,11 @@ class _BNLReLUFn(torch.autograd.Function):
         mu, rs, var = (torch.empty(C, device=x2.device) for _ in range(3))
         rm, rv, nbt, m = run if run is not None else (None, None, None, 0.0)
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        ws = _ws(lib, P, C, x2.device)  # (held by its name until the launches are enqueued)
         _lib.check(lib.esr_bn_lrelu_fwd(x2.data_ptr(), P, C, gamma.data_ptr(), beta.data_ptr(), eps, slope,
                                         y.data_ptr(), mu.data_ptr(), rs.data_ptr(), var.data_ptr(),
-                                        _ws(lib, P, C, x2.device).data_ptr(), ptr(rm), ptr(rv), ptr(nbt), m,
-                                        _stream(x2)), 'esr_bn_lrelu_fwd')
+                                        ws.data_ptr(), ptr(rm), ptr(rv), ptr(nbt), m, _stream(x2)),
+                   'esr_bn_lrelu_fwd')
         ctx.save_for_backward(x2, gamma, beta, mu, rs)
         ctx.slope = slope
         ctx.mark_non_differentiable(mu, var)
@@ -57,9 +58,10 @@ class _BNLReLUBwdFn(torch.autograd.Function):
         P, C = x2.shape
         gx = torch.empty_like(x2)
         sums2 = torch.empty(2, C, device=x2.device)
+        ws = _ws(lib, P, C, x2.device)
         _lib.check(lib.esr_bn_lrelu_bwd(x2.data_ptr(), gy.data_ptr(), P, C, gamma.data_ptr(), beta.data_ptr(),
                                         mu.data_ptr(), rs.data_ptr(), slope, gx.data_ptr(), sums2.data_ptr(),
-                                        _ws(lib, P, C, x2.device).data_ptr(), _stream(x2)), 'esr_bn_lrelu_bwd')
+                                        ws.data_ptr(), _stream(x2)), 'esr_bn_lrelu_bwd')
         ctx.save_for_backward(x2, gamma, beta, gy, mu, rs, sums2)
         ctx.slope = slope
         return gx, sums2[1].clone(), sums2[0].clone()
@@ -71,12 +73,13 @@ class _BNLReLUBwdFn(torch.autograd.Function):
         P, C = x2.shape
         g_x, g_gy = torch.empty_like(x2), torch.empty_like(x2)
         g_gamma = torch.empty(C, device=x2.device)
-        ggx = ggx.contiguous() if ggx is not None else None
-        ptr = lambda t: None if t is None else t.contiguous().data_ptr()  # noqa: E731
+        ggx, ggg, ggb = (None if t is None else t.contiguous() for t in (ggx, ggg, ggb))
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        ws = _ws(lib, P, C, x2.device)
         _lib.check(lib.esr_bn_lrelu_bwd2(x2.data_ptr(), gy.data_ptr(), ptr(ggx), ptr(ggg), ptr(ggb), P, C,
                                          gamma.data_ptr(), beta.data_ptr(), mu.data_ptr(), rs.data_ptr(), ctx.slope,
                                          sums2.data_ptr(), g_x.data_ptr(), g_gy.data_ptr(), g_gamma.data_ptr(),
-                                         _ws(lib, P, C, x2.device).data_ptr(), _stream(x2)), 'esr_bn_lrelu_bwd2')
+                                         ws.data_ptr(), _stream(x2)), 'esr_bn_lrelu_bwd2')
         return g_x, g_gamma, None, g_gy, None, None, None
 
 

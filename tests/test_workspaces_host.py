@@ -8,7 +8,7 @@ import weakref
 import pytest
 import torch
 
-from esr_amd import _lib, act8, gn
+from esr_amd import _lib, act8, bn, gn
 
 
 class Storages:
@@ -57,6 +57,7 @@ def stub(monkeypatch):
     monkeypatch.setattr(_lib, 'load', lambda: lib)
     monkeypatch.setattr(act8, 'on', lambda dev: contextlib.nullcontext())
     monkeypatch.setattr(act8, 'stream', lambda dev: 0)
+    monkeypatch.setattr(bn, '_stream', lambda t: None)
     monkeypatch.setattr(act8, 'check_dev', lambda what, *ts: ts[0].device)
     gn._ws_bytes.cache_clear()
     yield lib
@@ -73,3 +74,14 @@ def test_group_norm_workspaces(stub, ck, out8):
     gx, gw, gb = torch.autograd.grad(y.sum(), (x, w, b), create_graph=True)
     torch.autograd.grad(gx.sum() + gw.sum() + gb.sum(), (x, w))
     assert [n for n, _ in stub.calls if 'lrelu' in n] == ['esr_gn_lrelu_fwd', 'esr_gn_lrelu_bwd', 'esr_gn_lrelu_bwd2']
+
+
+def test_batch_norm_workspaces(stub):
+    """bn_lrelu, with upstream gradients of dγ and dβ that are expanded scalars: their copies live as long (released while
+    the arguments were evaluated, dβ's took dγ's memory)."""
+    m = torch.nn.BatchNorm2d(8)
+    stub.storages.seen.clear()  # (its parameters are other objects on the memory that torch.empty gave)
+    x = torch.randn(2, 8, 4, 4).contiguous(memory_format=torch.channels_last).requires_grad_()
+    gx, gw, gb = torch.autograd.grad(bn.bn_lrelu(x, m, 0.2).sum(), (x, m.weight, m.bias), create_graph=True)
+    torch.autograd.grad(gx.sum() + 2 * gw.sum() + 3 * gb.sum(), (x, m.weight))
+    assert [n for n, _ in stub.calls if 'lrelu' in n] == ['esr_bn_lrelu_fwd', 'esr_bn_lrelu_bwd', 'esr_bn_lrelu_bwd2']
