@@ -60,6 +60,7 @@ def phase(sf):
 def downscale(x, w, sf, zero_pad=False):
     """y[i, j] = sum_uv w[u, v] x[sf*i+ph+u-k//2, sf*j+ph+v-k//2], x edge-padded (or zero-padded); H, W % sf == 0."""
     _check(x, w)
+    w = w.contiguous()
     lead, (H, W) = x.shape[:-2], x.shape[-2:]
     if H % sf or W % sf:
         raise RuntimeError('esr_amd.cem_ops.downscale: image size %dx%d is not a multiple of %d' % (H, W, sf))
@@ -71,7 +72,7 @@ def downscale(x, w, sf, zero_pad=False):
     P, _, Hp, Wp = xp.shape
     y = torch.empty(P, 3, Hp // sf, Wp // sf, device=x.device, dtype=torch.float32)
     _lib.check(_lib.load().esr_cem_down(xp.data_ptr(), None, y.data_ptr(), P, Hp // sf, Wp // sf, sf, phase(sf),
-                                        w.contiguous().data_ptr(), k, 1, _stream(x)), 'esr_cem_down')
+                                        w.data_ptr(), k, 1, _stream(x)), 'esr_cem_down')
     if c:
         y = y[:, :, c:c + H // sf, c:c + W // sf]
     return _unplanes(y, n, lead)
@@ -81,6 +82,7 @@ def upscale(x, w, sf, zero_pad=False, crop=0):
     """y = xcorr(pad(S), w) with S = x zero-stuffed at the stride phase on the ×sf grid, pad = edge (clamp) or zero,
     then `crop` HR pixels removed from every side (fused: the cropped border is never computed)."""
     _check(x, w)
+    w = w.contiguous()
     lead, (h, wd) = x.shape[:-2], x.shape[-2:]
     k = w.shape[0]
     c = -(-(k // 2) // sf) if zero_pad else 0
@@ -94,13 +96,14 @@ def upscale(x, w, sf, zero_pad=False, crop=0):
     zero = torch.zeros(P, 3, sf * hp, sf * wp, device=x.device, dtype=torch.float32)
     y = torch.empty(P, 3, sf * hp - 2 * M, sf * wp - 2 * M, device=x.device, dtype=torch.float32)
     _lib.check(_lib.load().esr_cem_up_add(xp.data_ptr(), zero.data_ptr(), y.data_ptr(), P, hp, wp, sf, phase(sf),
-                                          w.contiguous().data_ptr(), k, M, _stream(x)), 'esr_cem_up_add')
+                                          w.data_ptr(), k, M, _stream(x)), 'esr_cem_up_add')
     return _unplanes(y, n, lead)
 
 
 def filter_same(x, w, zero_pad=True):
     """xcorr(pad(x), w) at the input resolution ('same' size); zero or edge (replicate) padding."""
     _check(x, w)
+    w = w.contiguous()
     lead, (H, W) = x.shape[:-2], x.shape[-2:]
     k = w.shape[0]
     p = k // 2 if zero_pad else 0
@@ -109,7 +112,7 @@ def filter_same(x, w, zero_pad=True):
     xp, n = _planes(x)
     P, _, Hp, Wp = xp.shape
     y = torch.empty_like(xp)
-    _lib.check(_lib.load().esr_cem_inv(xp.data_ptr(), y.data_ptr(), P, Hp, Wp, w.contiguous().data_ptr(), k,
+    _lib.check(_lib.load().esr_cem_inv(xp.data_ptr(), y.data_ptr(), P, Hp, Wp, w.data_ptr(), k,
                                        _stream(x)), 'esr_cem_inv')
     if p:
         y = y[:, :, p:p + H, p:p + W]

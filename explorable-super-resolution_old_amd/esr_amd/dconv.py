@@ -506,7 +506,8 @@ def _df_fwd(xh, w, b, slope, flags, mask=None, out=None):
     """esr_dfirst_fwd: [B][H][W][3] -> [B][H][W][64] (flags: LeakyReLU / mask by lrelu'(mask) / accumulate into out)."""
     B, H, W, _ = xh.shape
     y = out if out is not None else torch.empty(B, H, W, 64, device=xh.device, dtype=torch.float32)
-    _lib.check(_lib.load().esr_dfirst_fwd(xh.data_ptr(), B, H, W, w.contiguous().data_ptr(), _ptr(b), slope, flags,
+    w = w.contiguous()
+    _lib.check(_lib.load().esr_dfirst_fwd(xh.data_ptr(), B, H, W, w.data_ptr(), _ptr(b), slope, flags,
                                           _ptr(mask), y.data_ptr(), _stream(xh)), 'esr_dfirst_fwd')
     return y
 
@@ -522,7 +523,8 @@ def _df_bwd(xh, gy, mask, slope, w, need_x, need_w):
         nb = lib.esr_dfirst_bwd_blocks(B, H, W)
         part = torch.empty(nb * _DF_NW, device=gy.device, dtype=torch.float32)
     st = _stream(gy)
-    _lib.check(lib.esr_dfirst_bwd(_ptr(xh), gy.data_ptr(), _ptr(mask), slope, B, H, W, w.contiguous().data_ptr(),
+    w = w.contiguous()
+    _lib.check(lib.esr_dfirst_bwd(_ptr(xh), gy.data_ptr(), _ptr(mask), slope, B, H, W, w.data_ptr(),
                                   _ptr(gx), _ptr(part), st), 'esr_dfirst_bwd')
     gwb = None
     if need_w:

@@ -1130,17 +1130,18 @@ def cem_apply(lib, cem, gen, lr, Bn, H, W, M, stream, sf=SF):
     for t, n in ((wd, 'DownscaleOP'), (wi, 'Conv_LR_with_Inv_hTh_OP'), (wu, 'Upscale_OP')):
         _require_device(t, n + ' filter')
     kd, ki = wd.shape[-1], wi.shape[-1]
+    wd, wi, wu = (t[0, 0].contiguous() for t in (wd, wi, wu))
     r = torch.empty(Bn, 3, H, W, device=dev, dtype=torch.float32)
     q = torch.empty_like(r)
     if hasattr(lib, 'keep'):  # recording an op list: the intermediates must outlive this call
-        lib.keep += [r, q]
+        lib.keep += [r, q, wd, wi, wu]
     out = torch.empty(Bn, 3, sf * H - 2 * M, sf * W - 2 * M, device=dev, dtype=torch.float32)
     _lib.check(lib.esr_cem_down(gen.data_ptr(), lr.data_ptr(), r.data_ptr(), Bn, H, W, sf, ph,
-                                wd[0, 0].contiguous().data_ptr(), kd, 0, stream), 'esr_cem_down')
-    _lib.check(lib.esr_cem_inv(r.data_ptr(), q.data_ptr(), Bn, H, W, wi[0, 0].contiguous().data_ptr(), ki, stream),
+                                wd.data_ptr(), kd, 0, stream), 'esr_cem_down')
+    _lib.check(lib.esr_cem_inv(r.data_ptr(), q.data_ptr(), Bn, H, W, wi.data_ptr(), ki, stream),
                'esr_cem_inv')
     _lib.check(lib.esr_cem_up_add(q.data_ptr(), gen.data_ptr(), out.data_ptr(), Bn, H, W, sf, ph,
-                                  wu[0, 0].contiguous().data_ptr(), kd, M, stream), 'esr_cem_up_add')
+                                  wu.data_ptr(), kd, M, stream), 'esr_cem_up_add')
     return out
 
 

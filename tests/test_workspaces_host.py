@@ -3,7 +3,6 @@ arguments are evaluated goes back to the allocator before the launch is enqueued
 next argument's) can be given the same memory.  The library is stubbed; the calls run on CPU tensors."""
 import contextlib
 import gc
-import weakref
 
 import pytest
 import torch
@@ -12,11 +11,11 @@ from esr_amd import _lib, act8, bn, gn
 
 
 class Storages:
-    """Weak references to the tensors that torch.empty and Tensor.contiguous hand out, by address; the storages are kept,
-    so that no address comes twice."""
+    """The storages that torch.empty and Tensor.contiguous hand out, by address.  They are kept, so that no address comes
+    twice; one that nothing but this list holds has been released."""
 
     def __init__(self, monkeypatch):
-        self.seen, self.kept = [], []
+        self.seen = {}
         for owner, name in ((torch, 'empty'), (torch.Tensor, 'contiguous')):
             self.wrap(monkeypatch, owner, name)
 
@@ -26,10 +25,12 @@ class Storages:
         def call(*a, **k):
             k.pop('device', None)
             t = real(*a, **k)
-            self.seen.append((t.data_ptr(), weakref.ref(t)))
-            self.kept.append(t.untyped_storage())
+            self.seen[t.data_ptr()] = t.untyped_storage()
             return t
         monkeypatch.setattr(owner, name, call)
+
+    def released(self, p):
+        return p in self.seen and torch._C._storage_Use_Count(self.seen[p]._cdata) == 1
 
 
 class Stub:
@@ -39,13 +40,14 @@ class Stub:
         self.storages, self.calls = storages, []
 
     def __getattr__(self, name):
+        if not name.startswith('esr_'):
+            raise AttributeError(name)
+
         def entry(*args):
             gc.collect()
-            living = {p for p, r in self.storages.seen if r() is not None}
-            known = {p for p, _ in self.storages.seen if p}
             for i, a in enumerate(args):
-                if isinstance(a, int) and a in known:
-                    assert a in living, '%s: the memory of argument %d was released before the launch' % (name, i)
+                assert not (isinstance(a, int) and self.storages.released(a)), \
+                    '%s: the memory of argument %d was released before the launch' % (name, i)
             self.calls.append((name, args))
             return 1 << 10 if name.endswith(('_bytes', '_floats', '_blocks')) else 0
         return entry
@@ -80,8 +82,35 @@ def test_batch_norm_workspaces(stub):
     """bn_lrelu, with upstream gradients of dγ and dβ that are expanded scalars: their copies live as long (released while
     the arguments were evaluated, dβ's took dγ's memory)."""
     m = torch.nn.BatchNorm2d(8)
-    stub.storages.seen.clear()  # (its parameters are other objects on the memory that torch.empty gave)
     x = torch.randn(2, 8, 4, 4).contiguous(memory_format=torch.channels_last).requires_grad_()
     gx, gw, gb = torch.autograd.grad(bn.bn_lrelu(x, m, 0.2).sum(), (x, m.weight, m.bias), create_graph=True)
     torch.autograd.grad(gx.sum() + 2 * gw.sum() + 3 * gb.sum(), (x, m.weight))
     assert [n for n, _ in stub.calls if 'lrelu' in n] == ['esr_bn_lrelu_fwd', 'esr_bn_lrelu_bwd', 'esr_bn_lrelu_bwd2']
+
+
+def test_first_block_and_cem_filters(stub, monkeypatch):
+    """Weights and filters that are not contiguous (a network moved to channels last, a transposed filter) are copied; the
+    copies live until the launches are enqueued."""
+    from esr_amd import cem_ops, dconv, engine
+    for m in (dconv, cem_ops):
+        monkeypatch.setattr(m, '_stream', lambda t: None)
+    monkeypatch.setattr(cem_ops, '_check', lambda *ts: None)
+    monkeypatch.setattr(engine, '_require_device', lambda *a: None)
+    w = torch.randn(64, 3, 3, 3).to(memory_format=torch.channels_last)
+    x, gy = torch.randn(1, 6, 5, 3), torch.randn(1, 6, 5, 64)
+    dconv._df_fwd(x, w, None, 0.2, 1)
+    dconv._df_bwd(x, gy, gy, 0.2, w, True, True)
+    f, img = torch.randn(7, 7).t(), torch.randn(3, 16, 16)
+    cem_ops.downscale(img, f, 4)
+    cem_ops.upscale(img, f, 4)
+    cem_ops.filter_same(img, f)
+
+    def layer():
+        op = type('Op', (), {})()
+        op.Filter_OP = type('Filter', (), {'weight': torch.randn(3, 1, 7, 7).transpose(2, 3)})()
+        return op
+    cem = type('Cem', (), {'DownscaleOP': layer(), 'Conv_LR_with_Inv_hTh_OP': layer(), 'Upscale_OP': layer()})()
+    engine.cem_apply(stub, cem, torch.randn(1, 3, 32, 32), torch.randn(1, 3, 8, 8), 1, 8, 8, 0, None)
+    names = [n for n, _ in stub.calls]
+    want = {'dfirst_fwd': 1, 'dfirst_bwd': 1, 'cem_down': 2, 'cem_inv': 2, 'cem_up_add': 2}
+    assert {n: names.count('esr_' + n) for n in want} == want
