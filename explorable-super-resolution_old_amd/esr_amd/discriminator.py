@@ -24,6 +24,7 @@ import math
 import os
 
 import torch.nn as nn
+from torch.nn.modules.module import _has_any_global_hook
 
 from . import act8
 from .bn import bn_lrelu, lrelu_nhwc
@@ -104,6 +105,12 @@ class Discriminator_VGG_128_(nn.Module):
         return _run(self.classifier, _run(self.features, x))
 
 
+def _hooked(*mods):
+    """Whether calling one of the modules runs a hook (its own, or one for all modules)."""
+    return _has_any_global_hook() or any(m._forward_pre_hooks or m._forward_hooks or m._backward_pre_hooks or
+                                         m._backward_hooks for m in mods)
+
+
 def _run(seq, x):
     """seq(x), with every training-mode BatchNorm2d -> LeakyReLU pair (conv_block's norm + act) run as the fused HIP
     layer of bn.py (forward, backward and double backward), the first conv block (3 -> 64 3x3 conv + LeakyReLU) on the
@@ -123,10 +130,11 @@ def _run(seq, x):
             i += 2
             continue
         elif isinstance(m, HipConv2d):
-            x = m(x, x8)
+            x = m(x) if x8 is None or _hooked(m) else m(x, x8)  # (a hook may change x, not x8)
         elif isinstance(m, HipGroupNorm) and isinstance(nxt, nn.LeakyReLU):
             after = mods[i + 2] if i + 2 < len(mods) else None
-            if isinstance(after, HipConv2d) and after.keeps8():  # its input's 8-bit blocks from the norm's own pass
+            # its input's 8-bit blocks from the norm's own pass
+            if isinstance(after, HipConv2d) and after.keeps8() and not _hooked(after):
                 x, x8 = m.lrelu(x, nxt.negative_slope, True)
             else:
                 x, x8 = m.lrelu(x, nxt.negative_slope), None

@@ -1,0 +1,85 @@
+"""How the discriminator walks its layers (discriminator._run): which calls the modules get, and that hooks fire as in
+nn.Sequential.  The layers' kernels are replaced by plain functions, so the walk runs on the CPU."""
+import torch
+import torch.nn as nn
+
+from esr_amd import act8, discriminator
+from esr_amd.dconv import HipConv2d
+from esr_amd.gn import HipGroupNorm
+
+
+class Conv(HipConv2d):
+    """Records what it is called with; adds 1."""
+
+    def forward(self, x, x8=None):
+        self.got = (x, x8)
+        return x + 1
+
+
+class PlainConv(HipConv2d):
+    """A subclass whose forward takes the input alone."""
+
+    def forward(self, x):
+        self.got = x
+        return x + 1
+
+
+class Norm(HipGroupNorm):
+    """2x in place of the norm; its blocks are the output they belong to."""
+
+    def lrelu(self, x, slope, out8=False):
+        y = torch.where(x > 0, 2 * x, 2 * slope * x)
+        return (y, ('blocks of', y)) if out8 else y
+
+
+def net(conv=Conv, ck='int8'):
+    mods = [conv(4, 4, 3, padding=1), Norm(2, 4, checkpoint=ck), nn.LeakyReLU(0.5), conv(4, 4, 3, padding=1)]
+    for m in mods:
+        if isinstance(m, HipConv2d):
+            m.act_checkpoint = ck
+    return nn.Sequential(*mods)
+
+
+X = torch.tensor([-3.0, 2.0, 5.0, -1.0]).view(1, 4, 1, 1)
+WANT = torch.tensor([-2.0, 6.0, 12.0, 0.0]).view(1, 4, 1, 1)  # what reaches the second convolution
+
+
+def test_blocks_go_to_the_convolution_behind_the_norm():
+    seq = net()
+    discriminator._run(seq, X)
+    assert torch.equal(seq[3].got[0], WANT) and seq[3].got[1][1] is seq[3].got[0] and seq[0].got[1] is None
+
+
+def test_convolutions_without_blocks_get_the_input_alone():
+    for ck in (None, 'int8'):
+        seq = net(PlainConv, ck)
+        if ck:
+            seq[3].weight.requires_grad_(False)  # keeps nothing
+        discriminator._run(seq, X)
+        assert torch.equal(seq[3].got, WANT)
+    seq = net(ck=None)
+    seen = []
+    seq[3].register_forward_pre_hook(lambda m, args: seen.append(args))
+    discriminator._run(seq, X)
+    assert [len(a) for a in seen] == [1]
+
+
+def test_a_hook_that_changes_the_input_leaves_no_blocks_of_the_old_one():
+    seq = net()
+    seq[3].register_forward_pre_hook(lambda m, args: (args[0] * 3,))
+    discriminator._run(seq, X)
+    assert torch.equal(seq[3].got[0], 3 * WANT) and seq[3].got[1] is None
+    # in place: the blocks that the norm's pass would have written are those of the values before
+    seq = net()
+    seq[3].register_forward_pre_hook(lambda m, args: (args[0].mul_(3),))
+    discriminator._run(seq, X)
+    assert torch.equal(seq[3].got[0], 3 * WANT) and seq[3].got[1] is None
+    # a hook for all modules
+    h = nn.modules.module.register_module_forward_pre_hook(
+        lambda m, args: (args[0] * 3,) if isinstance(m, Conv) else None)
+    try:
+        seq = net()
+        discriminator._run(seq, X)
+    finally:
+        h.remove()
+    assert seq[3].got[1] is None
