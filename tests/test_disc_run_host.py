@@ -33,7 +33,7 @@ class Norm(HipGroupNorm):
 
 
 def net(conv=Conv, ck='int8'):
-    mods = [conv(4, 4, 3, padding=1), Norm(2, 4, checkpoint=ck), nn.LeakyReLU(0.5), conv(4, 4, 3, padding=1)]
+    mods = [conv(4, 4, 3, padding=1), Norm(2, 4, checkpoint=ck), nn.LeakyReLU(0.5, True), conv(4, 4, 3, padding=1)]
     for m in mods:
         if isinstance(m, HipConv2d):
             m.act_checkpoint = ck
@@ -83,3 +83,22 @@ def test_a_hook_that_changes_the_input_leaves_no_blocks_of_the_old_one():
     finally:
         h.remove()
     assert seq[3].got[1] is None
+
+
+def test_hooks_of_the_norm_and_its_activation_fire():
+    want = discriminator._run(net(), X)
+    for at in (1, 2):
+        for kind in ('register_forward_hook', 'register_forward_pre_hook'):
+            seq, seen = net(), []
+            getattr(seq[at], kind)(lambda m, *args: seen.append(m))
+            assert torch.equal(discriminator._run(seq, X), want) and seen == [seq[at]]
+    seq = net()
+    seq[1].register_forward_hook(lambda m, args, y: -y)  # a hook that changes the norm's result
+    out = discriminator._run(seq, X)
+    plain = nn.functional.leaky_relu(-2 * (X + 1), 0.5) + 1
+    assert torch.equal(out, plain) and seq[3].got[1] is None
+    seq, seen = net(), []
+    x = X.clone().requires_grad_()
+    seq[1].register_full_backward_hook(lambda m, gi, go: seen.append(m))
+    discriminator._run(seq, x).sum().backward()
+    assert seen == [seq[1]]
