@@ -411,6 +411,18 @@ class DConvAct8Fn(torch.autograd.Function):
         return gx, None, None, None, gw, gb, None, None, None, None
 
 
+class _ValuesFn(torch.autograd.Function):
+    """(carrier, codes, exps) -> the blocks' values, whose gradient goes on to the carrier (and so to x)."""
+
+    @staticmethod
+    def forward(ctx, carrier, codes, exps):
+        return act8.Act8.of(codes, exps, carrier.shape).unpack()
+
+    @staticmethod
+    def backward(ctx, g):
+        return g, None, None
+
+
 class WgradAct8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, carrier, gy, codes, exps, k, s, p, prec=None):
@@ -425,7 +437,7 @@ class WgradAct8Fn(torch.autograd.Function):
         ggw = ggw.contiguous()
         g_x = DgradFn.apply(gy, ggw, k, s, p, carrier.shape[1], carrier.shape[2], prec) \
             if ctx.needs_input_grad[0] else None
-        g_gy = DConvFn.apply(act8.Act8.of(codes, exps, carrier.shape).unpack(), ggw, None, k, s, p, prec) \
+        g_gy = DConvAct8Fn.apply(_ValuesFn.apply(carrier, codes, exps), carrier, codes, exps, ggw, None, k, s, p, prec) \
             if ctx.needs_input_grad[1] else None
         return g_x, g_gy, None, None, None, None, None, None
 

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from esr_amd import bn  # noqa: E402
+from esr_amd import act8, bn, dconv  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +28,28 @@ def test_batch_norm_expanded_upstreams(gpu_device):
     got = torch.autograd.grad(0.5 * gs[0].sum() + 2.0 * gs[1].sum() - 3.0 * gs[2].sum(), (x, m.weight))
     for p, q in zip(got, want):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize('k,s,p', [(3, 1, 1), (4, 2, 1)])
+def test_conv_checkpoint_third_order(gpu_device, k, s, p):
+    """A convolution that keeps its input in 8 bits, on values that the blocks hold exactly: every term of its third
+    derivatives is there (the plain layer's, up to what two evaluations of its products differ by)."""
+    torch.manual_seed(k)
+    m = dconv.HipConv2d(64, 32, k, stride=s, padding=p).to(gpu_device)
+    x0 = act8.pack(torch.randn(2, 10, 12, 64, device=gpu_device)).unpack().permute(0, 3, 1, 2)
+    gy0 = torch.randn_like(m(x0))
+    ups = [torch.randn_like(t) for t in (x0, m.weight, m.bias)]
+    ups2 = [torch.randn_like(t) for t in (x0, m.weight, gy0)]
+    res = []
+    for ck in (None, 'int8'):
+        m.act_checkpoint = ck
+        x, gy = x0.detach().requires_grad_(), gy0.detach().requires_grad_()
+        u = [t.detach().requires_grad_() for t in ups]
+        first = torch.autograd.grad(m(x), (x, m.weight, m.bias), gy, create_graph=True)
+        second = torch.autograd.grad(sum((a * b).sum() for a, b in zip(first, u)), (x, m.weight, gy), create_graph=True)
+        res.append(first + second + torch.autograd.grad(sum((a * b).sum() for a, b in zip(second, ups2)),
+                                                        [x, m.weight, gy] + u))
+    for i, (a, b) in enumerate(zip(*res)):
+        # both split each operand into f16 pieces that keep 2^-21 of it or better; the sums have at most 2·10·12 = 240 or
+        # 64·k² = 1024 terms, each rounded by 2^-24 of a partial sum: sqrt(1024) of them in the mean
+        assert float((a - b).norm()) <= (2 * 2.0 ** -21 + 32 * 2.0 ** -24) * 4 * float(b.norm()) + 1e-12, i
