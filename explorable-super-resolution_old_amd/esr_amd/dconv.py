@@ -437,8 +437,8 @@ class WgradAct8Fn(torch.autograd.Function):
         ggw = ggw.contiguous()
         g_x = DgradFn.apply(gy, ggw, k, s, p, carrier.shape[1], carrier.shape[2], prec) \
             if ctx.needs_input_grad[0] else None
-        g_gy = DConvAct8Fn.apply(_ValuesFn.apply(carrier, codes, exps), carrier, codes, exps, ggw, None, k, s, p, prec) \
-            if ctx.needs_input_grad[1] else None
+        g_gy = DConvAct8Fn.apply(_ValuesFn.apply(carrier, codes, exps), carrier, codes, exps, ggw, None, k, s, p,
+                                 prec) if ctx.needs_input_grad[1] else None
         return g_x, g_gy, None, None, None, None, None, None
 
 
@@ -558,6 +558,7 @@ class _DFirstFn(torch.autograd.Function):
     def forward(ctx, xh, w, b, slope, keep8=False):
         y = _df_fwd(xh, w, b, slope, _DF_LRELU)
         ctx.slope, ctx.keep8 = slope, keep8
+        ctx.set_materialize_grads(False)  # no gradients of zeros for y's blocks
         if not keep8:
             ctx.save_for_backward(xh, w, y)
             return y
@@ -567,7 +568,9 @@ class _DFirstFn(torch.autograd.Function):
         return y, y8.codes, y8.exps
 
     @staticmethod
-    def backward(ctx, gy, *_unused):
+    def backward(ctx, gy, *_blocks):
+        if gy is None:
+            return (None,) * 5
         xh, w, *y = ctx.saved_tensors
         y, y8 = (None, tuple(y)) if ctx.keep8 else (y[0], None)
         nx, nw, nb = ctx.needs_input_grad[:3]

@@ -77,6 +77,7 @@ class _GNLReLUFn(torch.autograd.Function):
                                                     _p(y8[1]), ws.data_ptr(), act8.stream(dev)), 'esr_gn_lrelu_fwd')
         ctx.save_for_backward(x if carrier is None else carrier, codes, exps, gamma, beta, stat)
         ctx.geom = (G, slope)
+        ctx.set_materialize_grads(False)  # no gradients of zeros for y's blocks
         if not out8:
             return y
         ctx.mark_non_differentiable(*y8)
@@ -84,6 +85,8 @@ class _GNLReLUFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gy, *_blocks):
+        if gy is None:
+            return (None,) * 8
         src, codes, exps, gamma, beta, stat = ctx.saved_tensors
         gy = _nhwc(gy)
         if torch.is_grad_enabled():

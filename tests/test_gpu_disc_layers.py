@@ -51,5 +51,6 @@ def test_conv_checkpoint_third_order(gpu_device, k, s, p):
                                                         [x, m.weight, gy] + u))
     for i, (a, b) in enumerate(zip(*res)):
         # both split each operand into f16 pieces that keep 2^-21 of it or better; the sums have at most 2·10·12 = 240 or
-        # 64·k² = 1024 terms, each rounded by 2^-24 of a partial sum: sqrt(1024) of them in the mean
+        # 64·k² = 1024 terms, each rounded by 2^-24 of a partial sum: sqrt(1024) of them in the mean; a third derivative
+        # goes through up to two such products, and both evaluations err: 4
         assert float((a - b).norm()) <= (2 * 2.0 ** -21 + 32 * 2.0 ** -24) * 4 * float(b.norm()) + 1e-12, i

@@ -114,3 +114,28 @@ def test_first_block_and_cem_filters(stub, monkeypatch):
     names = [n for n, _ in stub.calls]
     want = {'dfirst_fwd': 1, 'dfirst_bwd': 1, 'cem_down': 2, 'cem_inv': 2, 'cem_up_add': 2}
     assert {n: names.count('esr_' + n) for n in want} == want
+
+
+@pytest.mark.parametrize('ck', [None, 'int8'])
+def test_blocks_get_no_gradients_of_zeros(stub, monkeypatch, ck):
+    """Layers that hand on their output's 8-bit blocks beside it: the backward makes no gradient for them (zeros of their
+    size in every backward)."""
+    from torch.profiler import ProfilerActivity, profile
+
+    from esr_amd import dconv
+    monkeypatch.setattr(dconv, '_stream', lambda t: None)
+    monkeypatch.setattr(dconv, '_check_dev', lambda *ts: None)
+    x = torch.randn(2, 8, 4, 4).contiguous(memory_format=torch.channels_last).requires_grad_()
+    y, _ = gn.group_norm_lrelu(x, 4, checkpoint=ck, out8=True)
+    outs = [(y, x)]
+    if ck:
+        conv = dconv.HipConv2d(3, 64, 3, padding=1)
+        conv.act_checkpoint = ck
+        img = torch.randn(1, 3, 6, 5).contiguous(memory_format=torch.channels_last).requires_grad_()
+        outs.append((dconv.dfirst_lrelu8(img, conv, 0.2)[0], img))
+    for out, leaf in outs:
+        gy = torch.randn_like(out)
+        with profile(activities=[ProfilerActivity.CPU]) as prof:
+            torch.autograd.grad(out, leaf, gy)
+        names = {e.name for e in prof.events()}
+        assert not names & {'aten::zeros', 'aten::zeros_like'}, names
