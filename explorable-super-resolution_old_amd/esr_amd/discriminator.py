@@ -132,9 +132,9 @@ def _run(seq, x):
         elif isinstance(m, HipConv2d):
             x = m(x) if x8 is None or _hooked(m) else m(x, x8)  # (a hook may change x, not x8)
         elif isinstance(m, HipGroupNorm) and isinstance(nxt, nn.LeakyReLU):
-            if _hooked(m, nxt):  # the norm alone and its LeakyReLU, by their calls (a hooked output may not be written to)
+            if _hooked(m, nxt):  # the norm alone and its LeakyReLU, by their calls
                 y = m(x)
-                x, x8 = nxt(y.clone() if nxt.inplace else y), None
+                x, x8 = nxt(y.clone() if nxt.inplace else y), None  # (a hooked output may not be written to)
                 i += 2
                 continue
             after = mods[i + 2] if i + 2 < len(mods) else None

@@ -171,7 +171,15 @@ class HipGroupNorm(nn.GroupNorm):
         super().__init__(num_groups, num_channels, eps=eps, affine=affine)
         self.checkpoint = act8.check_mode(checkpoint)
 
+    def check(self, x):
+        """Refuses an input of one value per (sample, group), as nn.InstanceNorm2d does: what the layer gives is its bias
+        then, whatever the value, and no gradient passes it."""
+        if x.dim() == 4 and x.shape[2] * x.shape[3] * (self.num_channels // self.num_groups) == 1:
+            raise ValueError('HipGroupNorm: one value per sample and group in %s, %d groups: its norm is 0 for every input'
+                             % (tuple(x.shape), self.num_groups))
+
     def lrelu(self, x, slope, out8=False):
+        self.check(x)
         return group_norm_lrelu(x, self.num_groups, self.weight, self.bias, self.eps, slope, self.checkpoint, out8)
 
     def forward(self, x):

@@ -102,3 +102,38 @@ def test_hooks_of_the_norm_and_its_activation_fire():
     seq[1].register_full_backward_hook(lambda m, gi, go: seen.append(m))
     discriminator._run(seq, x).sum().backward()
     assert seen == [seq[1]]
+
+
+def test_a_group_of_one_value_is_refused():
+    """128 x 128 crops through four strides leave the classifier's 8x8 layer a 1 x 1 map: an instance norm there makes
+    the score the same for every input and its gradient 0."""
+    import pytest
+
+    from esr_amd.discriminator import Discriminator_VGG_128_
+    for layer, x in ((HipGroupNorm(4, 4), torch.zeros(2, 4, 1, 1)), (HipGroupNorm(1, 1), torch.zeros(2, 1, 1, 1)),
+                     (HipGroupNorm(4, 4, affine=False).eval(), torch.zeros(2, 4, 1, 1))):
+        for call in (layer, lambda t, layer=layer: layer.lrelu(t, 0.2)):
+            with pytest.raises(ValueError, match='one value'):
+                call(x)
+    # the discriminator: shapes alone, the convolutions' of PyTorch and the norms' check
+    for norm, groups, refused in (('instance', 32, True), ('group', 32, False), ('group', 100, True)):
+        netD = Discriminator_VGG_128_(3, 64, norm_type=norm, nb=8, num_2_strides=4, norm_groups=groups)
+
+        def walk(seq, x):
+            for m in seq.children():
+                if isinstance(m, nn.Sequential):
+                    x = walk(m, x)
+                elif isinstance(m, HipConv2d):
+                    x = torch.empty(x.shape[0], m.out_channels, *((n + 2 * m.padding[0] - m.kernel_size[0]) //
+                                                                  m.stride[0] + 1 for n in x.shape[2:]))
+                elif isinstance(m, HipGroupNorm):
+                    m.check(x)
+            return x
+
+        def score():
+            return walk(netD.classifier, walk(netD.features, torch.empty(2, 3, 128, 128))).shape
+        if refused:
+            with pytest.raises(ValueError, match='one value'):
+                score()
+        else:
+            assert score() == (2, 1, 1, 1)

@@ -54,3 +54,17 @@ def test_conv_checkpoint_third_order(gpu_device, k, s, p):
         # 64·k² = 1024 terms, each rounded by 2^-24 of a partial sum: sqrt(1024) of them in the mean; a third derivative
         # goes through up to two such products, and both evaluations err: 4
         assert float((a - b).norm()) <= (2 * 2.0 ** -21 + 32 * 2.0 ** -24) * 4 * float(b.norm()) + 1e-12, i
+
+
+def test_score_depends_on_the_input_or_is_refused(gpu_device):
+    """128 x 128 crops through four strides: the head's map is 1 x 1.  Group norm's critic answers to its input there;
+    instance norm's could not, and is refused."""
+    from esr_amd.discriminator import Discriminator_VGG_128_
+    torch.manual_seed(1)
+    x = torch.rand(2, 3, 128, 128, device=gpu_device).requires_grad_()
+    mk = lambda norm: Discriminator_VGG_128_(3, 64, norm_type=norm, nb=8, num_2_strides=4).to(gpu_device)  # noqa: E731
+    y = mk('group')(x)
+    gx, = torch.autograd.grad(y.sum(), x)
+    assert y.shape == (2, 1, 1, 1) and float(y[0]) != float(y[1]) and float(gx[0].norm()) > 0 and float(gx[1].norm()) > 0
+    with pytest.raises(ValueError, match='one value'):
+        mk('instance')(x)
