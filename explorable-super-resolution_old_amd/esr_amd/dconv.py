@@ -285,7 +285,10 @@ def _wgrad_act8_bytes(*geom):
 
 def conv_wgrad_act8(x8, gy, k, s, p):
     """conv_wgrad from an input kept in 8 bits: x8 = act8.Act8 of the NHWC input, gy NHWC [B][Ho][Wo][Co] fp32; exact
-    products of the codes' values with gy to fp32 accuracy (csrc/esr_wgrad8.hip)."""
+    products of the codes' values with gy to fp32 accuracy (csrc/esr_wgrad8.hip).  The result has no graph (HipConv2d
+    with act_checkpoint is the differentiable layer): a gy that asks for its gradient is refused."""
+    if gy.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError('conv_wgrad_act8 has no derivative: detach the gradient, or call it under torch.no_grad()')
     act8.check_dev('dconv', gy)
     if gy.device != x8.codes.device:
         raise RuntimeError('conv_wgrad_act8: the input is on %s, the gradient on %s' % (x8.codes.device, gy.device))

@@ -58,3 +58,14 @@ def test_orders(plain, k, s, p):
         for i, (a, r) in enumerate(zip(orders(conv), want)):
             torch.testing.assert_close(a, r, rtol=1e-12, atol=1e-12 * float(r.detach().abs().max()),
                                        msg=lambda m, i=i: '%d: %s' % (i, m))
+
+
+def test_weight_gradient_call_refuses_to_lose_a_gradient():
+    x8 = act8.Act8(torch.zeros(1, 4, 4, 16, dtype=torch.int8), torch.zeros(1, 4, 4, 1, dtype=torch.uint8), 8)
+    gy = torch.zeros(1, 4, 4, 8, requires_grad=True)
+    with pytest.raises(RuntimeError, match='no derivative'):
+        dconv.conv_wgrad_act8(x8, gy, 3, 1, 1)
+    with pytest.raises(RuntimeError, match='ROCm device'):
+        dconv.conv_wgrad_act8(x8, gy.detach(), 3, 1, 1)
+    with torch.no_grad(), pytest.raises(RuntimeError, match='ROCm device'):
+        dconv.conv_wgrad_act8(x8, gy, 3, 1, 1)
