@@ -548,6 +548,9 @@ inline bool aligned(std::initializer_list<const void *> ptrs) {  // to 16 bytes
     return true;
 }
 
+// a grid's third dimension (C > 65535·256 without 16-byte accesses exceeds it; gn_small's chunks are its first)
+inline bool grid_ok(const GnP &p) { return !p.blocks || p.chunks <= 65535; }
+
 // the fewest channels of whole groups and, unless it is all of them, whole 8-bit blocks
 int chunk_of(int32_t C, int32_t Cg) {
     int64_t s = Cg;
@@ -638,6 +641,7 @@ extern "C" int esr_gn_lrelu_fwd(const float *x, int64_t N, int64_t HW, int32_t C
     const hipStream_t st = (hipStream_t)stream;
     const int V = C % 4 == 0 && aligned({x, y}) ? 4 : 1;
     GnP p = params(V, N, HW, C, G, gamma, beta, slope);
+    if (!grid_ok(p)) return ESR_EINVAL;
     p.x = x; p.eps = eps;
     pass<0>(p, V, codes || ycodes, GnOut{y, nullptr, nullptr, nullptr, codes, ycodes, exps, yexps}, (double *)ws, nullptr,
             stat, st);
@@ -652,6 +656,7 @@ extern "C" int esr_gn_lrelu_bwd(const float *x, const int8_t *codes, const uint8
     const hipStream_t st = (hipStream_t)stream;
     const int V = C % 4 == 0 && aligned({x, gy, gx}) ? 4 : 1;
     GnP p = params(V, N, HW, C, G, gamma, beta, slope);
+    if (!grid_ok(p)) return ESR_EINVAL;
     p.x = x; p.codes = codes; p.exps = exps; p.gy = gy; p.stat = stat;
     double *partial = (double *)ws, *grp = partial + N * p.splits * 3 * C + N * 3 * C;
     pass<1>(p, V, !x, GnOut{gx, nullptr, g_gamma, g_beta, nullptr, nullptr, nullptr, nullptr}, partial, sums_, grp, st);
@@ -668,6 +673,7 @@ extern "C" int esr_gn_lrelu_bwd2(const float *x, const int8_t *codes, const uint
     const hipStream_t st = (hipStream_t)stream;
     const int V = C % 4 == 0 && aligned({x, gy, u, g_x, g_gy}) ? 4 : 1;
     GnP p = params(V, N, HW, C, G, gamma, beta, slope);
+    if (!grid_ok(p)) return ESR_EINVAL;
     p.x = x; p.codes = codes; p.exps = exps; p.gy = gy; p.u = u; p.gga = gg_gamma; p.ggb = gg_beta; p.stat = stat;
     p.sums = sums_;
     double *partial = (double *)ws, *su = partial + N * p.splits * 3 * C, *grp = su + N * 3 * C;

@@ -484,7 +484,8 @@ int esr_dconv_wgrad_act8(const int8_t *codes, const uint8_t *exps, int64_t B, in
 
 /* ---- GroupNorm + LeakyReLU, channels last (esr_gn.hip) -------------------------------------------------------------
  * x, y, gy, ... [N][HW][C] fp32; G groups of C/G channels; gamma, beta [C] or NULL (1, 0; G = C without them is
- * instance norm); N <= 65535, C <= 2^24.  y = lrelu_slope(γ·(x − μ)·r + β), r = 1/sqrt(v + eps) over each (sample, group).
+ * instance norm); N <= 65535, C <= 2^24 (65535·256 where C or a base is not a multiple of 4 values).
+ * y = lrelu_slope(γ·(x − μ)·r + β), r = 1/sqrt(v + eps) over each (sample, group).
  * esr_gn_lrelu_fwd writes y and stat [N][G][2] (μ and r, float64) and, where codes / exps are given, x in 8-bit
  *   blocks (above) whose pre-activations keep the sign x's have (a code moves one step where rounding would change it,
  *   so that its error is less than a step; at e = 254 it stays where that step leads past the largest float);
