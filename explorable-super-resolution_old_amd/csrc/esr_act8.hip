@@ -98,21 +98,33 @@ __global__ __launch_bounds__(NT) void act8_unpack_kernel(const int8_t *codes, co
     }
 }
 
-// the rows and the grid; false where the sizes do not fit it
-bool plan(int64_t P, int32_t C, int V, Rows &r, dim3 &grid) {
+// the rows; false where the sizes do not fit the kernels
+bool plan(int64_t P, int32_t C, int V, Rows &r, int &chunks) {
     if (P <= 0 || C <= 0 || P > (1LL << 46) / C) return false;
     const bool flat = C % act8::BLK == 0;  // rows of one block each
     r.P = flat ? P * (C / act8::BLK) : P;
     r.C = flat ? act8::BLK : C;
     r.nb = (r.C + act8::BLK - 1) / act8::BLK;
     r.cp = act8::pitch(r.C);
-    const int lanes = r.nb * (act8::BLK / V), chunks = (lanes + NT - 1) / NT;
+    const int lanes = r.nb * (act8::BLK / V);
+    chunks = (lanes + NT - 1) / NT;
     r.lanes = lanes < NT ? lanes : NT;
     r.rpi = NT / r.lanes;
-    const long long blocks = (r.P + (long long)r.rpi * UN - 1) / (r.rpi * UN);
-    if (blocks > 0x7fffffffLL || chunks > 65535) return false;
-    grid = dim3((unsigned)blocks, (unsigned)chunks);
-    return true;
+    return chunks <= 65535;
+}
+
+// launch(grid, part, first row) over all rows: a grid's first dimension ends below 2^32 threads, so that long tensors take
+// several launches (of 2^23 workgroups: 2^28 rows of one channel, 2^30 of 32)
+template <typename F>
+int parts(const Rows &r, int chunks, F launch) {
+    const long long per = (long long)r.rpi * UN, most = per << 23;
+    for (long long p0 = 0; p0 < r.P; p0 += most) {
+        Rows part = r;
+        part.P = r.P - p0 < most ? r.P - p0 : most;
+        launch(dim3((unsigned)((part.P + per - 1) / per), (unsigned)chunks), part, p0);
+        if (hipGetLastError() != hipSuccess) return ESR_ELAUNCH;
+    }
+    return ESR_OK;
 }
 
 inline bool quads(const void *f32, int C) { return C % 4 == 0 && (uintptr_t)f32 % 16 == 0; }
@@ -123,12 +135,12 @@ extern "C" int esr_act8_pack(const float *x, int64_t P, int32_t C, int8_t *codes
     if (!x || !codes || !exps || C <= 0 || (uintptr_t)codes % 16) return ESR_EINVAL;
     const int V = quads(x, C) ? 4 : 1;
     Rows r;
-    dim3 grid;
-    if (!plan(P, C, V, r, grid)) return ESR_EINVAL;
-    const hipStream_t st = (hipStream_t)stream;
-    if (V == 4) hipLaunchKernelGGL(act8_pack_kernel<4>, grid, dim3(NT), 0, st, x, r, codes, exps);
-    else hipLaunchKernelGGL(act8_pack_kernel<1>, grid, dim3(NT), 0, st, x, r, codes, exps);
-    return hipGetLastError() == hipSuccess ? ESR_OK : ESR_ELAUNCH;
+    int chunks;
+    if (!plan(P, C, V, r, chunks)) return ESR_EINVAL;
+    return parts(r, chunks, [&](dim3 grid, const Rows &t, long long p0) {
+        hipLaunchKernelGGL(V == 4 ? act8_pack_kernel<4> : act8_pack_kernel<1>, grid, dim3(NT), 0, (hipStream_t)stream,
+                           x + p0 * r.C, t, codes + p0 * r.cp, exps + p0 * r.nb);
+    });
 }
 
 extern "C" int esr_act8_unpack(const int8_t *codes, const uint8_t *exps, int64_t P, int32_t C, float *x,
@@ -136,10 +148,10 @@ extern "C" int esr_act8_unpack(const int8_t *codes, const uint8_t *exps, int64_t
     if (!x || !codes || !exps || C <= 0 || (uintptr_t)codes % 16) return ESR_EINVAL;
     const int V = quads(x, C) ? 4 : 1;
     Rows r;
-    dim3 grid;
-    if (!plan(P, C, V, r, grid)) return ESR_EINVAL;
-    const hipStream_t st = (hipStream_t)stream;
-    if (V == 4) hipLaunchKernelGGL(act8_unpack_kernel<4>, grid, dim3(NT), 0, st, codes, exps, r, x);
-    else hipLaunchKernelGGL(act8_unpack_kernel<1>, grid, dim3(NT), 0, st, codes, exps, r, x);
-    return hipGetLastError() == hipSuccess ? ESR_OK : ESR_ELAUNCH;
+    int chunks;
+    if (!plan(P, C, V, r, chunks)) return ESR_EINVAL;
+    return parts(r, chunks, [&](dim3 grid, const Rows &t, long long p0) {
+        hipLaunchKernelGGL(V == 4 ? act8_unpack_kernel<4> : act8_unpack_kernel<1>, grid, dim3(NT), 0, (hipStream_t)stream,
+                           codes + p0 * r.cp, exps + p0 * r.nb, t, x + p0 * r.C);
+    });
 }

@@ -53,6 +53,7 @@ def test_conv_checkpoint_third_order(gpu_device, k, s, p):
         # both split each operand into f16 pieces that keep 2^-21 of it or better; the sums have at most 2·10·12 = 240 or
         # 64·k² = 1024 terms, each rounded by 2^-24 of a partial sum: sqrt(1024) of them in the mean; a third derivative
         # goes through up to two such products, and both evaluations err: 4
+        a, b = a.detach(), b.detach()
         assert float((a - b).norm()) <= (2 * 2.0 ** -21 + 32 * 2.0 ** -24) * 4 * float(b.norm()) + 1e-12, i
 
 
