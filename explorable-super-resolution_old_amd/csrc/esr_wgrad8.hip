@@ -26,6 +26,7 @@
 #include "esr_act8.h"
 #include "esr_amd.h"
 #include "esr_knobs.h"
+#include "esr_wgrad8_map.h"
 
 namespace {
 
@@ -82,11 +83,9 @@ __global__ __launch_bounds__(256 * TG, 2) void wgrad8_kernel(WgP p) {
     __shared__ unsigned s_red[4 * TG][2];
     __shared__ int s_flag[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hl = lane >> 5;
-    // workgroups of one split share its pixels: they go to one XCD (workgroup ids go round the 8 XCDs)
-    const int work = p.nci * p.nco * p.groups, j8 = blockIdx.x >> 3;
-    const int split = j8 / work * 8 + (blockIdx.x & 7);
-    if (split >= p.splits) return;
-    int w = j8 % work;
+    const wgrad8::Place place = wgrad8::place((int)blockIdx.x, p.splits, p.nci * p.nco * p.groups);
+    const int split = place.split;
+    int w = place.item;
     const int cob = w % p.nco;
     w /= p.nco;
     const int cib = w % p.nci, grp = w / p.nci;
@@ -355,6 +354,9 @@ __global__ __launch_bounds__(NT) void wgrad8_reduce_rows(const float *partial, i
     }
 }
 
+// input channels of a workgroup of wgrad8_reduce_rows
+constexpr int reduced(int T) { return T < 64 ? 64 / T : 1; }
+
 struct Geo {
     int kind;  // 0: 3×3, 1: 4×4 stride 2, 2: 4×4 stride 1, 3: 8×8, 4: tap by tap
     WgP p;
@@ -403,13 +405,16 @@ bool geometry(int64_t B, int32_t Hs, int32_t Ws, int32_t cin, int32_t MH, int32_
         }
     }
     p.splits = (p.tiles + p.per_split - 1) / p.per_split;
-    return (long long)(p.splits + 7) / 8 * 8 * work <= 0x7fffffffLL;
+    // (below 2^32 threads of a grid, the reduction's by rows among them)
+    const int cb = reduced(k * k);
+    return p.splits * work * (g.kind == 1 ? 2 * NT : NT) < 1LL << 32 &&
+           (long long)((cout + 31) / 32) * ((cin + cb - 1) / cb) * NT < 1LL << 32;
 }
 
 template <bool G4>
 void run(const Geo &g, hipStream_t st) {
     const WgP &p = g.p;
-    const dim3 grid((unsigned)((p.splits + 7) / 8 * 8 * p.nci * p.nco * p.groups)), block(NT);
+    const dim3 grid((unsigned)(p.splits * p.nci * p.nco * p.groups)), block(NT);
     switch (g.kind) {
         case 0: hipLaunchKernelGGL((wgrad8_kernel<3, 3, 1, 1, G4>), grid, block, 0, st, p); break;
         case 1: hipLaunchKernelGGL((wgrad8_kernel<2, 4, 2, 2, G4>), grid, dim3(2 * NT), 0, st, p); break;
@@ -440,7 +445,7 @@ extern "C" int esr_dconv_wgrad_act8(const int8_t *codes, const uint8_t *exps, in
     p.codes = codes; p.exps = exps; p.dy = dy; p.partial = (float *)ws;
     if (cout % 4 == 0 && (uintptr_t)dy % 16 == 0) run<true>(g, st);
     else run<false>(g, st);
-    const int T = k * k, nco = (cout + 31) / 32, cb = T < 64 ? 64 / T : 1;
+    const int T = k * k, nco = (cout + 31) / 32, cb = reduced(T);
     const long long rows = (long long)nco * ((cin + cb - 1) / cb);
     if (rows >= 256)  // enough workgroups without cutting the splits (64->512 8x8 of 8 images: 75 -> 43 us in all)
         hipLaunchKernelGGL(wgrad8_reduce_rows, dim3((unsigned)rows), dim3(NT), 0, st, p.partial, p.splits, T, cin, cout,
