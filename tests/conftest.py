@@ -1,3 +1,4 @@
+import gc
 import glob
 import json
 import os
@@ -62,6 +63,21 @@ def gpu_device():
     if not torch.cuda.is_available():
         pytest.skip('no ROCm device')
     return torch.device('cuda:0')
+
+
+# tests that compare torch.cuda.memory_allocated() with what their tensors hold
+MEASURE_MEMORY = ('test_checkpoint_frees_the_input', 'test_discriminator_with_checkpoints')
+
+
+@pytest.fixture(autouse=True)
+def no_cached_blocks(request):
+    """memory_allocated() counts the blocks that the allocator hands out, and it hands out a cached block that is up to
+    1 MB too large whole: what such a test measures would depend on what ran before it.  They start without cached blocks."""
+    if getattr(request.node, 'originalname', None) in MEASURE_MEMORY:
+        import torch
+        if torch.cuda.is_available():
+            gc.collect()
+            torch.cuda.empty_cache()
 
 
 @pytest.fixture(scope='session')

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from esr_amd import act8, bn, dconv  # noqa: E402
+from esr_amd import act8, bn, dconv, gn  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -66,6 +66,25 @@ def test_score_depends_on_the_input_or_is_refused(gpu_device):
     mk = lambda norm: Discriminator_VGG_128_(3, 64, norm_type=norm, nb=8, num_2_strides=4).to(gpu_device)  # noqa: E731
     y = mk('group')(x)
     gx, = torch.autograd.grad(y.sum(), x)
+    y = y.detach()
     assert y.shape == (2, 1, 1, 1) and float(y[0]) != float(y[1]) and float(gx[0].norm()) > 0 and float(gx[1].norm()) > 0
     with pytest.raises(ValueError, match='one value'):
         mk('instance')(x)
+
+
+def test_checkpoint_holds_blocks_and_statistics(gpu_device):
+    """What a forward with a checkpoint leaves allocated beside its input and output, in the bytes that were asked for (the
+    allocator may hand out larger blocks that it has cached: one is left for it here)."""
+    requested = lambda: torch.cuda.memory_stats()['requested_bytes.all.current']  # noqa: E731
+    x = cl(torch.randn(4, 64, 128, 128, device=gpu_device))
+    codes, exps = x.numel(), x.numel() // 32
+    gn.group_norm_lrelu(x, 32)
+    src = (x * 2.0).requires_grad_()
+    for ck, kept in ((None, 4 * x.numel()), ('int8', codes + exps + 4)):
+        spare = torch.empty(codes + (7 << 17), dtype=torch.uint8, device=gpu_device)
+        base = requested()
+        del spare
+        y = gn.group_norm_lrelu(src * 1.0, 32, checkpoint=ck)  # the product's storage lives on only if it is saved
+        held = requested() - base + codes + (7 << 17) - 4 * x.numel()
+        assert held == kept + 2 * 4 * 32 * 8, (ck, held)  # μ and r of every (sample, group), float64
+        del y
