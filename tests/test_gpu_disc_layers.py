@@ -7,6 +7,8 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import disc_ref  # noqa: E402
+import test_disc_ref_host as T  # noqa: E402
 from esr_amd import act8, bn, dconv, gn  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -88,3 +90,45 @@ def test_checkpoint_holds_blocks_and_statistics(gpu_device):
         held = requested() - base + codes + (7 << 17) - 4 * x.numel()
         assert held == kept + 2 * 4 * 32 * 8, (ck, held)  # μ and r of every (sample, group), float64
         del y
+
+
+@pytest.mark.parametrize('norm', ['batch', 'group', 'instance'])
+def test_discriminator_with_checkpoints_against_its_definition(gpu_device, norm):
+    """A WGAN-GP step of the discriminator that keeps its activations in 8 bits: every gradient is the float64 network's that
+    reads the blocks' values in its backward and double backward (the host test of that network says what would show)."""
+    netD = T.discriminator(norm, 'int8')
+    want = T.step(disc_ref.network(netD))
+    got = [t.detach() for t in T.critic_step(netD.to(gpu_device), *T.data(), torch.float32, gpu_device)]
+    assert [tuple(t.shape) for t in got] == [tuple(t.shape) for t in want]
+    far = T.apart(got, want, norm)
+    assert far <= T.BOUND[norm], far
+
+
+@pytest.mark.parametrize('bad', [None, float('nan'), float('inf')])
+def test_first_block_checkpoint_is_exact(gpu_device, bad):
+    """The first block keeps its output's sign in 8 bits: output, gradients and double backward bit for bit those of the
+    block that keeps its output."""
+    torch.manual_seed(2)
+    conv = dconv.HipConv2d(3, 64, 3, padding=1).to(gpu_device)
+    x0 = cl(torch.rand(2, 3, 21, 18, device=gpu_device))
+    if bad is not None:
+        x0[1, 2, 5, 7] = bad
+    gy0 = cl(torch.randn(2, 64, 21, 18, device=gpu_device))
+    ups = [torch.randn_like(t) for t in (x0, conv.weight, conv.bias)]
+    res = []
+    for ck in (None, 'int8'):
+        conv.act_checkpoint = ck
+        x, gy = x0.detach().requires_grad_(), gy0.detach().requires_grad_()
+        y, y8 = dconv.dfirst_lrelu8(x, conv, 0.2)
+        assert (y8 is not None) == bool(ck)
+        first = torch.autograd.grad(y, (x, conv.weight, conv.bias), gy, create_graph=True)
+        second = torch.autograd.grad(sum((a * b).sum() for a, b in zip(first, ups)), (x, gy, conv.weight))
+        res.append([y, *first, *second])
+    if ck and bad is None:
+        assert torch.equal(y8.codes, act8.pack(y.detach().permute(0, 2, 3, 1)).codes)
+    for i, (a, b) in enumerate(zip(*res)):
+        a, b = a.detach(), b.detach()
+        if bad is None:
+            assert torch.equal(a, b), i
+        else:  # the whole block of a non-finite value reads back as NaN: at its pixels the slope of the others is lost
+            assert torch.equal(a[0], b[0]) or i in (2, 3, 6), i
