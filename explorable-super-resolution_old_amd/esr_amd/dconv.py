@@ -431,7 +431,10 @@ class WgradAct8Fn(torch.autograd.Function):
     def forward(ctx, carrier, gy, codes, exps, k, s, p, prec=None):
         ctx.save_for_backward(carrier, gy, codes, exps)
         ctx.geom = (k, s, p, prec)
-        return conv_wgrad_act8(act8.Act8.of(codes, exps, carrier.shape), gy, k, s, p)
+        x8 = act8.Act8.of(codes, exps, carrier.shape)
+        if (prec or PRECISION) == 'x3':
+            return conv_wgrad_act8(x8, gy, k, s, p)
+        return conv_wgrad(x8.unpack(), gy, k, s, p, prec)  # another arithmetic asked for: that of the blocks' values
 
     @staticmethod
     def backward(ctx, ggw):

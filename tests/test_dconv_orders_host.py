@@ -69,3 +69,24 @@ def test_weight_gradient_call_refuses_to_lose_a_gradient():
         dconv.conv_wgrad_act8(x8, gy.detach(), 3, 1, 1)
     with torch.no_grad(), pytest.raises(RuntimeError, match='ROCm device'):
         dconv.conv_wgrad_act8(x8, gy, 3, 1, 1)
+
+
+@pytest.mark.parametrize('prec,kernel', [(None, 'act8'), ('x3', 'act8'), ('x6', 'x6'), ('f32', 'f32')])
+def test_precision_of_the_weight_gradient(plain, monkeypatch, prec, kernel):
+    """A layer (or the module) set to another arithmetic than x3 has it for the weight gradient of its blocks too."""
+    ran = []
+    gw = torch.ones(4, 5, 3, 3, dtype=torch.float64)
+    monkeypatch.setattr(dconv, 'conv_wgrad', lambda x, gy, k, s, p, prec=None: ran.append(prec) or gw)
+    monkeypatch.setattr(dconv, 'conv_wgrad_act8', lambda x8, gy, k, s, p: ran.append('act8') or gw)
+    x = torch.ones(1, 6, 6, 5, dtype=torch.float64)
+    codes, exps = torch.ones(1, 6, 6, 16, dtype=torch.int8), torch.full((1, 6, 6, 1), 132, dtype=torch.uint8)
+    w = torch.ones(4, 5, 3, 3, dtype=torch.float64, requires_grad=True)
+    dconv.DConvAct8Fn.apply(x, x, codes, exps, w, None, 3, 1, 1, prec).sum().backward()
+    assert ran == [kernel]
+    if prec:
+        prev = dconv.set_precision(prec)
+        try:
+            dconv.DConvAct8Fn.apply(x, x, codes, exps, w, None, 3, 1, 1).sum().backward()
+        finally:
+            dconv.set_precision(prev)
+        assert ran == [kernel] * 2

@@ -132,3 +132,16 @@ def test_first_block_checkpoint_is_exact(gpu_device, bad):
             assert torch.equal(a, b), i
         else:  # the whole block of a non-finite value reads back as NaN: at its pixels the slope of the others is lost
             assert torch.equal(a[0], b[0]) or i in (2, 3, 6), i
+
+
+@pytest.mark.parametrize('prec', ['x6', 'f32'])
+def test_conv_checkpoint_in_another_precision(gpu_device, prec):
+    """The weight gradient of a layer set to x6 or f32 is that arithmetic's, of the blocks' values."""
+    torch.manual_seed(4)
+    m = dconv.HipConv2d(64, 32, 3, padding=1).to(gpu_device)
+    m.act_checkpoint, m.esr_precision = 'int8', prec
+    x = cl(torch.randn(2, 64, 14, 11, device=gpu_device))
+    gy = cl(torch.randn(2, 32, 14, 11, device=gpu_device))
+    gw, = torch.autograd.grad(m(x), m.weight, gy)
+    v = act8.pack(x.permute(0, 2, 3, 1)).unpack()
+    assert torch.equal(gw, dconv.conv_wgrad(v, gy.permute(0, 2, 3, 1), 3, 1, 1, prec))
