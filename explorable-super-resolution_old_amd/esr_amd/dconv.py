@@ -667,6 +667,10 @@ class HipConv2d(nn.Conv2d):
     Square kernel, equal stride and zero padding in both dimensions, no dilation / groups (what conv_block builds).
     Input: NCHW tensor (any memory format; channels-last avoids a copy); output: NCHW with channels-last storage."""
 
+    # 'int8': the input is kept for the weight gradient in 8 bits (act8.py).  (Of the class, for layers that were pickled
+    # without it.)
+    act_checkpoint = None
+
     def __init__(self, *args, **kwargs):
         super().__init__(*args, **kwargs)
         k, s, p = self.kernel_size, self.stride, self.padding
@@ -677,7 +681,6 @@ class HipConv2d(nn.Conv2d):
         # one 32-wide K step instead of one (mostly zero) K step per tap
         self._im2col = s[0] == 1 and self.in_channels * k[0] * k[1] <= 32 and self.in_channels < 8
         self.esr_precision = None  # this layer's precision ('x3' / 'x6' / 'f32'); None = the module default
-        self.act_checkpoint = None  # 'int8': the input is kept for the weight gradient in 8 bits (act8.py)
 
     def keeps8(self):
         """Whether a forward now keeps its input (the fused first block: its output) in 8 bits."""

@@ -137,3 +137,10 @@ def test_a_group_of_one_value_is_refused():
                 score()
         else:
             assert score() == (2, 1, 1, 1)
+
+
+def test_layers_saved_whole_before_they_had_checkpoints():
+    """A pickled discriminator's convolutions without the attribute keep fp32."""
+    m = HipConv2d(4, 4, 3, padding=1)
+    m.__dict__.pop('act_checkpoint', None)
+    assert m.act_checkpoint is None and not m.keeps8()
