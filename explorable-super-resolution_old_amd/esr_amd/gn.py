@@ -154,6 +154,8 @@ def group_norm_lrelu(x, groups, weight=None, bias=None, eps=1e-5, slope=0.2, che
     dev = act8.check_dev('gn', x, weight, bias)
     if B == 0:
         y = x * 1.0
+        for t in (weight, bias):  # (a gradient of zeros, as nn.GroupNorm's)
+            y = y if t is None else y * t.view(1, C, 1, 1)
         return (y, act8.Act8(*act8.empty_blocks((0, H, W, C), dev), C)) if out8 else y
     x = _nhwc(x)
     weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))

@@ -144,3 +144,18 @@ def test_layers_saved_whole_before_they_had_checkpoints():
     m = HipConv2d(4, 4, 3, padding=1)
     m.__dict__.pop('act_checkpoint', None)
     assert m.act_checkpoint is None and not m.keeps8()
+
+
+def test_empty_batch_has_gradients_of_zero(monkeypatch):
+    """No images: the norm's weight and bias get gradients of zero, as nn.GroupNorm's do, not none."""
+    from esr_amd import gn
+    monkeypatch.setattr(act8, 'check_dev', lambda what, *ts: ts[0].device)
+    for out8 in (False, True):
+        x = torch.zeros(0, 4, 3, 2, requires_grad=True)
+        w, b = torch.ones(4, requires_grad=True), torch.zeros(4, requires_grad=True)
+        y = gn.group_norm_lrelu(x, 2, w, b, out8=out8)
+        y = y[0] if out8 else y
+        assert y.shape == x.shape
+        gx, gw, gb = torch.autograd.grad(y.sum(), (x, w, b))
+        assert gx.shape == x.shape and torch.equal(gw, torch.zeros(4)) and torch.equal(gb, torch.zeros(4))
+    assert gn.group_norm_lrelu(x, 2).shape == x.shape
