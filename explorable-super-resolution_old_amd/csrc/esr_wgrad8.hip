@@ -19,10 +19,11 @@
 // first and expand second), so that one's expansion runs under the other's MFMAs.  The pixels are split over the grid,
 // the partial sums added in a fixed order by a second launch into torch's weight layout.
 //
-// The matrix cores' power bounds it: 3×3, 64 -> 128 channels, 16×152×152 pixels: about 105 us and 13 us of reduction, 1.04
-// PFLOP/s of f16 products (two for each of the definition's) where a large f16 matrix product reaches 1.2 on this card at
-// the clock it holds; 4×4 stride 2, 64 -> 64, 16×304×304: about 98 and 12 us.  LDS reads, expansion and loads run under
-// the products; a wait where the loads are issued, in place of where they are expanded, cost the 4×4 case 119 us.
+// 3×3, 64 -> 128 channels, 16×152×152 pixels: 108 to 120 us back to back and 14 us of reduction, 0.9 to 1.0 PFLOP/s of f16
+// products (two for each of the definition's) where a large f16 matrix product reaches 1.2 on this card; 4×4 stride 2,
+// 64 -> 64, 16×304×304: 103 to 113 and 12 us, 0.86 to 0.94.  The matrix pipes are busy 57 and 53 % of the cycles, at a
+// clock of 2.06 and 2.12 GHz; what the rest goes to (LDS reads, expansion, the first tile and the partial sums, which have
+// no MFMA beside them) has not been taken apart.
 #include "esr_act8.h"
 #include "esr_amd.h"
 #include "esr_knobs.h"

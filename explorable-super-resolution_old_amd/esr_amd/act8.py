@@ -4,8 +4,9 @@ A training step of the discriminator keeps every convolution's input and every n
 them: 8 bytes per activation value in fp32.  `pack` keeps 1 + 1/32: int8 codes that share a power-of-two step per 32
 channels of a pixel (error <= half a step <= max|x|/127 of the block; x > 0 is kept exactly, so LeakyReLU masks are: a
 positive value below half a step takes code 1).
-The backward kernels read the codes themselves: dconv.conv_wgrad_act8 (weight gradients) and gn.group_norm_lrelu
-(checkpoint='int8')."""
+The kernels of the weight gradients (dconv.conv_wgrad_act8) and of the norm's backward (gn.group_norm_lrelu with
+checkpoint='int8') read the codes themselves; the first block's LeakyReLU mask, a convolution's second derivative and weight
+gradients of another precision than x3 unpack them first."""
 import contextlib
 
 import torch

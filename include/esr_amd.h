@@ -471,6 +471,8 @@ int esr_bn_lrelu_bwd2(const float *x, const float *gy, const float *u, const flo
  *   gw[co][ci][ky][kx] = sum over b, Y, X of x[b, s*Y + ky - pad, s*X + kx - pad, ci] * dy[b, Y, X, co]
  * x [B][Hs][Ws][cin], dy [B][MH][MW][cout] fp32, MH = (Hs + 2·pad − k) / s + 1 (likewise MW), k <= 8, gw in torch's
  * layout; ws = esr_dconv_wgrad_act8_workspace_bytes(...) bytes, 16-byte aligned (ESR_EINVAL on bad arguments).
+ * Each product keeps dy to 2^-22 of it + 2^-36 of the largest |dy|, and x exactly in blocks down to 2^-27 of the largest
+ * (below, a block counts as zero), of those that a workgroup meets: 64 input x 64 output channels, a share of the pixels.
  * Sizes: Hs, Ws <= 65535, cin, cout <= 65536, an image's codes and four times its dy's values < 2^31 (ESR_EINVAL).  A
  * non-finite block makes the weights of its channels non-finite at every tap, a non-finite dy those of its output.
  * Deterministic. */
