@@ -145,3 +145,42 @@ def test_conv_checkpoint_in_another_precision(gpu_device, prec):
     gw, = torch.autograd.grad(m(x), m.weight, gy)
     v = act8.pack(x.permute(0, 2, 3, 1)).unpack()
     assert torch.equal(gw, dconv.conv_wgrad(v, gy.permute(0, 2, 3, 1), 3, 1, 1, prec))
+
+
+def test_two_threads(gpu_device):
+    """Two host threads with the layers on one stream, and on streams of their own: every result is the first call's."""
+    import threading
+    torch.manual_seed(6)
+    x0, gy0 = cl(torch.randn(2, 64, 40, 37, device=gpu_device)), cl(torch.randn(2, 32, 40, 37, device=gpu_device))
+    m = dconv.HipConv2d(64, 32, 3, padding=1).to(gpu_device)
+    m.act_checkpoint = 'int8'
+
+    def step(ck):
+        x = x0.detach().requires_grad_()
+        y, y8 = gn.group_norm_lrelu(x, 8, checkpoint=ck, out8=True)
+        out = m(y, y8)
+        gx, gw = torch.autograd.grad(out, (x, m.weight), gy0, create_graph=True)
+        return [t.detach() for t in (out, gx, gw)] + list(torch.autograd.grad(gx.pow(2).sum() + gw.sum(), (x, m.weight)))
+    want = {ck: step(ck) for ck in (None, 'int8')}
+    torch.cuda.synchronize()
+    got, errors = [], []
+
+    def run(ck, stream):
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(12):
+                    got.append((ck, step(ck)))
+                    torch.empty(1 << 16, device=gpu_device).fill_(float('nan'))  # a neighbour of the workspaces
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+    for streams in ([torch.cuda.current_stream()] * 2, [torch.cuda.Stream(), torch.cuda.Stream()]):
+        threads = [threading.Thread(target=run, args=a) for a in zip((None, 'int8'), streams)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+    assert not errors and len(got) == 48
+    for ck, outs in got:
+        for i, (a, b) in enumerate(zip(outs, want[ck])):
+            assert torch.equal(a, b), (ck, i)
