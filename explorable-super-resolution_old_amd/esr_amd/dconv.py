@@ -287,8 +287,8 @@ def conv_wgrad_act8(x8, gy, k, s, p):
     """conv_wgrad from an input kept in 8 bits: x8 = act8.Act8 of the NHWC input, gy NHWC [B][Ho][Wo][Co] fp32;
     products of the codes' values with gy to 2^-22 of gy + 2^-36 of the largest |gy| that a workgroup (64 x 64 channels, a
     share of the pixels) meets, exact in blocks down to 2^-27 of the largest there, below which they count as zero
-    (csrc/esr_wgrad8.hip).  The result has no graph (HipConv2d
-    with act_checkpoint is the differentiable layer): a gy that asks for its gradient is refused."""
+    (csrc/esr_wgrad8.hip).  The result has no graph (HipConv2d with act_checkpoint is the differentiable layer): a gy that
+    asks for its gradient is refused."""
     if gy.requires_grad and torch.is_grad_enabled():
         raise RuntimeError('conv_wgrad_act8 has no derivative: detach the gradient, or call it under torch.no_grad()')
     act8.check_dev('dconv', gy)
